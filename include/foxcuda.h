@@ -49,6 +49,9 @@ const char *foxcuda_version(void);
 /* Selects and checks the device (compute capability 10.x). */
 foxcuda_status foxcuda_init(int device);
 
+/* positions of a page of a paged K/V cache */
+#define FOXCUDA_KV_PAGE 64
+
 /* ---- kernel level (device pointers) ------------------------------------ */
 
 /* replaces fox_quantize_activations_i8 (include/fox/fox.h:342-343,
@@ -101,7 +104,9 @@ foxcuda_status foxcuda_gemm_kq_i8(int ggml_type, const int8_t *q, const float *a
                                   size_t n_cols, float *out, void *stream);
 /* Every tensor-core call above records a bounded wait that gave up in one
  * device error word per device (the outputs of that call are then not
- * valid). foxcuda_kernel_errors synchronises the stream, reports the word
+ * valid); the calls on the 4-bit cache and foxcuda_qk_norm_rope below record
+ * what their device arrays placed out of bounds there too.
+ * foxcuda_kernel_errors synchronises the stream, reports the word
  * and clears it. The first tensor-core call on a device looks the word up;
  * make it before any stream capture. */
 foxcuda_status foxcuda_kernel_errors(void *stream);
@@ -167,6 +172,90 @@ foxcuda_status foxcuda_attention(const float *q, const void *kcache, const void 
                                  int kv_type, uint32_t n_head, uint32_t n_head_kv,
                                  uint32_t head_dim, uint32_t n_ctx, uint32_t pos, int exact,
                                  float *out, void *stream);
+
+/* ---- a paged K/V cache in 4 bits, and what stands around it (device
+ * pointers; no upstream counterpart: upstream keeps one fp32 cache per
+ * context, src/forward.c:91-92) ---------------------------------------------
+ * The cache holds n_pages pages of FOXCUDA_KV_PAGE positions of every KV
+ * head: [page][kv_head][K block | V block], each block
+ * foxcuda_kv4_block_bytes(head_dim) bytes (4.5 bits a value). A block holds a
+ * code 0..15 per value and, per position and group of 64 dimensions, the
+ * fp16 pair (d, m) of x = m + d * code: m the largest fp16 not above the
+ * group's minimum, d the smallest fp16 with which level 15 reaches its
+ * maximum, the code the nearest level (ties to even). A value reads back
+ * within d / 2. Values beyond the range of fp16 are taken as its largest; a
+ * group that holds a NaN reads back as NaN.
+ *
+ * The rows of a call belong to sequences. Sequence s has the rows
+ * row_start[s] .. row_start[s+1]-1 of the row arrays, and they stand at the
+ * last of its kv_len[s] positions: row r at kv_len[s] - (row_start[s+1] - r).
+ * - A row whose position is negative has none: it is not written or read
+ *   back, and attends to nothing (its output is zeros).
+ * - Rows from row_start[n_seq] on are padding: left as they were.
+ * - Position p of sequence s lies in page table[s * table_stride + p / 64].
+ *   Entries behind a sequence's last page are not read. Sequences may share
+ *   pages that no row of the call is written to.
+ * - What the device arrays place outside their bounds (a page outside the
+ *   cache, a kv_len beyond table_stride pages) is skipped, the position as if
+ *   it were absent, and reported by foxcuda_kernel_errors. row_start must not
+ *   fall; it is held to n_rows.
+ * - head_dim 64, 128 or 256; at most 1024 sequences and 2^20 rows; the cache
+ *   and the row arrays 16-byte aligned, row strides (in elements) a multiple
+ *   of 16 bytes. No call allocates or synchronises, and each can be captured;
+ *   the first call on a device looks up its error word, so make that before
+ *   any capture. */
+typedef struct {
+    void          *cache;
+    const int32_t *table;      /* n_seq x table_stride */
+    const int32_t *row_start;  /* n_seq + 1 */
+    const int32_t *kv_len;     /* n_seq */
+    uint32_t n_pages, n_head_kv, head_dim;
+    uint32_t n_seq, table_stride;
+    uint32_t n_rows;           /* rows of the row arrays, padding included */
+} foxcuda_kv4;
+size_t         foxcuda_kv4_block_bytes(uint32_t head_dim);   /* 0: not covered */
+/* Quantises each row's K and V heads into its position. k and v are FOXCUDA_F32
+ * or FOXCUDA_F16 rows of n_head_kv * head_dim values. */
+foxcuda_status foxcuda_kv4_write(const foxcuda_kv4 *c, int ggml_type, const void *k, size_t k_stride,
+                                 const void *v, size_t v_stride, void *stream);
+/* The K and V values of each row's position, to rows of n_head_kv * head_dim
+ * FOXCUDA_F32 or FOXCUDA_F16 values. */
+foxcuda_status foxcuda_kv4_read(const foxcuda_kv4 *c, int ggml_type, void *k, void *v, void *stream);
+/* Each row's n_head query heads over positions 0..its own of its sequence
+ * (upstream attention_heads, src/forward.c:222-257, for many rows): q and out
+ * are rows of n_head * head_dim FOXCUDA_F32 or FOXCUDA_F16 values, q's
+ * q_stride elements apart. n_head / n_head_kv is 1, 2, 4 or 8; scale
+ * multiplies the scores (0: 1 / sqrt(head_dim)). The sums and softmax
+ * statistics are fp32, with fp16 queries the softmax weights are rounded to
+ * fp16. A row's result depends on its own sequence's lengths, not on the
+ * other sequences of the call. workspace holds
+ * foxcuda_kv4_attention_workspace() bytes (16-byte aligned; need not be
+ * initialised); calls that may run at the same time must not share it. */
+size_t         foxcuda_kv4_attention_workspace(uint32_t n_seq, uint32_t n_rows, uint32_t n_head,
+                                               uint32_t head_dim);
+foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4 *c, int ggml_type, const void *q, size_t q_stride,
+                                     uint32_t n_head, float scale, void *workspace,
+                                     size_t workspace_bytes, void *out, void *stream);
+/* Norms and rotation of the query and key heads in one pass. A row of x holds
+ * n_head query heads, then n_head_kv key heads (what follows, such as the
+ * value heads of a fused q|k|v row, is not read), FOXCUDA_F32 or FOXCUDA_F16.
+ * - q_norm and k_norm (head_dim floats each, or NULL): the head is RMS-normed,
+ *   x * (1 / sqrt(mean(x^2) + eps)) * w, before the rotation.
+ * - Row r is rotated by the angles of position pos[r]: (a, b) ->
+ *   (a cos - b sin, a sin + b cos), with cos and sin [n_pos][head_dim / 2].
+ *   The pairs are dimensions (2i, 2i + 1) as upstream's (src/ops.c:56-73), or
+ *   (i, i + head_dim / 2) with halves = 1.
+ * - A row with pos < 0 is padding: its outputs are left as they were. One with
+ *   pos >= n_pos is skipped and reported by foxcuda_kernel_errors.
+ * - q_out and k_out may be the rows of x that they come from (same strides),
+ *   and must not overlap x or one another otherwise. Without norms the values
+ *   are the decode step's rotation, bit for bit. */
+foxcuda_status foxcuda_qk_norm_rope(int ggml_type, const void *x, size_t x_stride, uint32_t n_rows,
+                                    uint32_t n_head, uint32_t n_head_kv, uint32_t head_dim,
+                                    const float *q_norm, const float *k_norm, float eps,
+                                    const float *cos, const float *sin, uint32_t n_pos, int halves,
+                                    const int32_t *pos, void *q_out, size_t q_stride, void *k_out,
+                                    size_t k_stride, void *stream);
 
 /* Integer partial sums exactly as upstream forms them, for bit-exact checks
  * (no single upstream entry point; the sums inside src/ternary.c:158-173,
@@ -274,7 +363,6 @@ foxcuda_status foxcuda_context_create(foxcuda_model *m, const foxcuda_context_co
  * are the contiguous cache's, bit for bit. A batch takes contexts that are
  * all contiguous or all from one pool. The pool outlives its contexts:
  * foxcuda_kv_pool_destroy answers FOXCUDA_ERR_ARG while any holds pages. */
-#define FOXCUDA_KV_PAGE 64
 typedef struct foxcuda_kv_pool foxcuda_kv_pool;
 foxcuda_status foxcuda_kv_pool_create(foxcuda_model *m, uint32_t n_pages, int kv_type,
                                       foxcuda_kv_pool **out);

@@ -14,6 +14,7 @@
 
 #include "../../include/foxcuda.h"
 #include "common.cuh"
+#include "host.cuh"
 #include "gemv.cuh"
 #include "ops.cuh"
 #include "pack.cuh"
@@ -28,71 +29,8 @@
 
 using namespace fox;
 
-// ---------------------------------------------------------------------------
-// errors: thread-local message, status codes of upstream fox_status
-
-static thread_local char g_err[512];
-
-static foxcuda_status fail(foxcuda_status st, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof g_err, fmt, ap);
-  va_end(ap);
-  return st;
-}
-
-static foxcuda_status cuda_fail(cudaError_t e, const char* what) {
-  return fail(e == cudaErrorMemoryAllocation ? FOXCUDA_ERR_NOMEM : FOXCUDA_ERR_INTERNAL,
-              "%s: %s", what, cudaGetErrorString(e));
-}
-
-#define CK(call, what)                                   \
-  do {                                                   \
-    cudaError_t e_ = (call);                             \
-    if (e_ != cudaSuccess) return cuda_fail(e_, what);   \
-  } while (0)
-
 extern "C" const char* foxcuda_last_error(void) { return g_err[0] ? g_err : "no error recorded"; }
 extern "C" const char* foxcuda_version(void) { return "foxcuda 0.1.0 (sm_100a)"; }
-
-static int sm_count(int dev) {
-  static int cached[64] = {0};
-  if (dev < 0 || dev >= 64) return 148;
-  if (!cached[dev]) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    cached[dev] = n;
-  }
-  return cached[dev];
-}
-
-static int current_sms() {
-  int d = 0;
-  cudaGetDevice(&d);
-  return sm_count(d);
-}
-
-// The dynamic shared-memory opt-in is a property of a kernel on one device,
-// so each launcher keeps its high-water mark per device (`marks` has one
-// slot per device ordinal). The attribute only ever rises, under a lock, so
-// two threads cannot leave it below a mark that another thread relies on.
-constexpr int kMaxDevices = 64;
-static std::mutex g_smem_mu;
-
-template <typename K>
-static cudaError_t opt_in_smem(K kern, size_t smem, size_t* marks) {
-  if (smem <= 48 * 1024) return cudaSuccess;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  std::lock_guard<std::mutex> lk(g_smem_mu);
-  if (smem <= marks[dev]) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  marks[dev] = smem;
-  return cudaSuccess;
-}
 
 extern "C" foxcuda_status foxcuda_init(int device) {
   int n = 0;
@@ -548,7 +486,7 @@ static __device__ int g_kernel_err;
 static std::mutex g_kernel_err_mu;
 static int* g_kernel_err_addr[kMaxDevices];
 
-static int* kernel_err_ptr() {
+int* fox::kernel_err_ptr() {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
   std::lock_guard<std::mutex> lock(g_kernel_err_mu);
@@ -567,6 +505,10 @@ extern "C" foxcuda_status foxcuda_kernel_errors(void* stream) {
   CK(cudaMemcpy(&code, p, 4, cudaMemcpyDeviceToHost), "kernel_errors");
   if (!code) return FOXCUDA_OK;
   CK(cudaMemset(p, 0, 4), "kernel_errors");
+  if (code == KERR_PAGES)
+    return fail(FOXCUDA_ERR_ARG, "device: a call named a row, position or page outside its arrays (a position "
+                "beyond the tables, a cached length beyond the block table, a page outside the cache); what lay "
+                "outside was skipped");
   return fail(FOXCUDA_ERR_INTERNAL, "device: a bounded wait of a kernel-level tensor-core call gave up "
               "(code %d); that call's output is not valid", code);
 }

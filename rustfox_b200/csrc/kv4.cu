@@ -1,0 +1,188 @@
+// The 4-bit paged K/V cache's entry points (include/foxcuda.h): argument
+// checks and launches of kv4.cuh and kv4_attn.cuh.
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "../../include/foxcuda.h"
+#include "common.cuh"
+#include "host.cuh"
+#include "kv4.cuh"
+#include "kv4_attn.cuh"
+
+using namespace fox;
+
+static_assert(FOXCUDA_KV_PAGE == KV_PAGE, "the header's page size is the kernels'");
+
+static bool kv4_hd_ok(uint32_t hd) { return hd == 64 || hd == 128 || hd == 256; }
+static bool kv4_type_ok(int t) { return t == T_F32 || t == T_F16; }
+static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+static bool stride_ok(size_t stride, size_t row, int type) {
+  return stride >= row && stride * (type == T_F32 ? 4 : 2) % 16 == 0 && stride <= ((size_t)1 << 32);
+}
+
+extern "C" size_t foxcuda_kv4_block_bytes(uint32_t head_dim) {
+  return kv4_hd_ok(head_dim) ? (size_t)kv4_block_bytes((int)head_dim) : 0;
+}
+
+// The checks every call on a cache makes; *none is set when there is no row.
+static foxcuda_status check_kv4(const foxcuda_kv4* c, int type, const char* what, Kv4Rows* r, bool* none) {
+  if (!c) return fail(FOXCUDA_ERR_ARG, "%s: null cache", what);
+  if (!kv4_type_ok(type)) return fail(FOXCUDA_ERR_UNSUPPORTED, "%s: rows of ggml type %d are not covered", what, type);
+  if (!kv4_hd_ok(c->head_dim))
+    return fail(FOXCUDA_ERR_UNSUPPORTED, "%s: head_dim %u is not 64, 128 or 256", what, c->head_dim);
+  if (!c->n_head_kv || c->n_head_kv > 1024) return fail(FOXCUDA_ERR_ARG, "%s: %u KV heads", what, c->n_head_kv);
+  if (c->n_seq > (uint32_t)KV4_MAX_SEQ || c->n_rows > (1u << 20))
+    return fail(FOXCUDA_ERR_ARG, "%s: %u sequences / %u rows are beyond %d and 2^20", what, c->n_seq, c->n_rows,
+                KV4_MAX_SEQ);
+  if (c->table_stride > (1u << 24) || c->n_pages > (uint32_t)INT_MAX)
+    return fail(FOXCUDA_ERR_ARG, "%s: %u pages a sequence / %u pages", what, c->table_stride, c->n_pages);
+  *none = c->n_rows == 0 || c->n_seq == 0;
+  if (*none) return FOXCUDA_OK;
+  if (!c->cache || !c->table || !c->row_start || !c->kv_len) return fail(FOXCUDA_ERR_ARG, "%s: null pointer", what);
+  if (!aligned16(c->cache)) return fail(FOXCUDA_ERR_ARG, "%s: the cache must be 16-byte aligned", what);
+  r->cache = static_cast<uint8_t*>(c->cache);
+  r->table = c->table; r->row_start = c->row_start; r->kv_len = c->kv_len;
+  r->n_pages = (int)c->n_pages; r->n_kv = (int)c->n_head_kv; r->n_seq = (int)c->n_seq;
+  r->table_stride = (int)c->table_stride; r->n_rows = (int)c->n_rows;
+  r->err = kernel_err_ptr();
+  return FOXCUDA_OK;
+}
+
+// f(type tag, head dimension) for the combination asked for.
+template <typename F>
+static cudaError_t by_type_hd(int type, uint32_t hd, F f) {
+  auto with = [&](auto tag) {
+    switch (hd) {
+      case 64: return f(tag, std::integral_constant<int, 64>());
+      case 128: return f(tag, std::integral_constant<int, 128>());
+      default: return f(tag, std::integral_constant<int, 256>());
+    }
+  };
+  return type == T_F32 ? with(float()) : with(__half());
+}
+
+extern "C" foxcuda_status foxcuda_kv4_write(const foxcuda_kv4* c, int type, const void* k, size_t k_stride,
+                                            const void* v, size_t v_stride, void* stream) {
+  Kv4WriteParams p{};
+  bool none = false;
+  foxcuda_status st = check_kv4(c, type, "kv4_write", &p.c, &none);
+  if (st || none) return st;
+  const size_t row = (size_t)c->n_head_kv * c->head_dim;
+  if (!k || !v) return fail(FOXCUDA_ERR_ARG, "kv4_write: null pointer");
+  if (!aligned16(k) || !aligned16(v) || !stride_ok(k_stride, row, type) || !stride_ok(v_stride, row, type))
+    return fail(FOXCUDA_ERR_ARG, "kv4_write: rows must be 16-byte aligned and at least a row apart");
+  p.k = k; p.v = v; p.k_stride = k_stride; p.v_stride = v_stride;
+  const size_t units = (size_t)c->n_rows * c->n_head_kv;
+  CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
+       kv4_write_kernel<decltype(tag), hd.value><<<(unsigned)((units + 7) / 8), 256, 0, (cudaStream_t)stream>>>(p);
+       return cudaGetLastError();
+     }), "kv4_write launch");
+  return FOXCUDA_OK;
+}
+
+extern "C" foxcuda_status foxcuda_kv4_read(const foxcuda_kv4* c, int type, void* k, void* v, void* stream) {
+  Kv4ReadParams p{};
+  bool none = false;
+  foxcuda_status st = check_kv4(c, type, "kv4_read", &p.c, &none);
+  if (st || none) return st;
+  if (!k || !v) return fail(FOXCUDA_ERR_ARG, "kv4_read: null pointer");
+  if (!aligned16(k) || !aligned16(v)) return fail(FOXCUDA_ERR_ARG, "kv4_read: rows must be 16-byte aligned");
+  p.k = k; p.v = v;
+  const size_t units = (size_t)c->n_rows * c->n_head_kv;
+  CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
+       kv4_read_kernel<decltype(tag), hd.value><<<(unsigned)((units + 7) / 8), 256, 0, (cudaStream_t)stream>>>(p);
+       return cudaGetLastError();
+     }), "kv4_read launch");
+  return FOXCUDA_OK;
+}
+
+extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x_stride, uint32_t n_rows,
+                                               uint32_t n_head, uint32_t n_head_kv, uint32_t head_dim,
+                                               const float* q_norm, const float* k_norm, float eps,
+                                               const float* cos, const float* sin, uint32_t n_pos, int halves,
+                                               const int32_t* pos, void* q_out, size_t q_stride, void* k_out,
+                                               size_t k_stride, void* stream) {
+  if (!kv4_type_ok(type)) return fail(FOXCUDA_ERR_UNSUPPORTED, "qk_norm_rope: rows of ggml type %d are not covered", type);
+  if (!kv4_hd_ok(head_dim)) return fail(FOXCUDA_ERR_UNSUPPORTED, "qk_norm_rope: head_dim %u is not 64, 128 or 256", head_dim);
+  if (!n_head || !n_head_kv || n_head > 1024 || n_head_kv > 1024)
+    return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: %u query heads / %u KV heads", n_head, n_head_kv);
+  if (halves != 0 && halves != 1) return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: halves %d", halves);
+  if (n_rows > (1u << 20) || n_pos > (uint32_t)INT_MAX)
+    return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: %u rows / %u positions", n_rows, n_pos);
+  if (n_rows == 0) return FOXCUDA_OK;
+  if (!x || !cos || !sin || !pos || !q_out || !k_out) return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: null pointer");
+  const size_t nq = (size_t)n_head * head_dim, nk = (size_t)n_head_kv * head_dim;
+  if (!aligned16(x) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(cos) || !aligned16(sin) ||
+      (q_norm && !aligned16(q_norm)) || (k_norm && !aligned16(k_norm)) || !stride_ok(x_stride, nq + nk, type) ||
+      !stride_ok(q_stride, nq, type) || !stride_ok(k_stride, nk, type))
+    return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: rows and tables must be 16-byte aligned, rows at least a row apart");
+  RopeParams p{};
+  p.x = x; p.pos = pos; p.q_norm = q_norm; p.k_norm = k_norm; p.cos = cos; p.sin = sin; p.q = q_out; p.k = k_out;
+  p.x_stride = x_stride; p.q_stride = q_stride; p.k_stride = k_stride;
+  p.n_rows = (int)n_rows; p.n_head = (int)n_head; p.n_kv = (int)n_head_kv; p.n_pos = (int)n_pos; p.halves = halves;
+  p.eps = eps; p.err = kernel_err_ptr();
+  const size_t units = (size_t)n_rows * (n_head + n_head_kv);
+  CK(by_type_hd(type, head_dim, [&](auto tag, auto hd) {
+       qk_norm_rope_kernel<decltype(tag), hd.value><<<(unsigned)((units + 7) / 8), 256, 0, (cudaStream_t)stream>>>(p);
+       return cudaGetLastError();
+     }), "qk_norm_rope launch");
+  return FOXCUDA_OK;
+}
+
+extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t n_seq, uint32_t n_rows, uint32_t n_head, uint32_t head_dim) {
+  if (!n_head || !kv4_hd_ok(head_dim)) return 0;
+  const size_t extra = (size_t)kv4_extra_slots((int)n_head, 8, current_sms());
+  return ((size_t)n_rows + n_seq * extra) * n_head * (head_dim + 4) * 4;
+}
+
+template <typename T, int HD, int NT>
+static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
+  using A = Kv4Attn<HD, NT>;
+  const size_t smem = A::smem_bytes(p.c.n_seq);
+  static size_t marks[kMaxDevices] = {};
+  cudaError_t e = opt_in_smem(kv4_attend_kernel<HD, T, NT>, smem, marks);
+  if (e != cudaSuccess) return e;
+  kv4_attend_kernel<HD, T, NT><<<p.sms, A::NW * 32, smem, s>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if (p.c.table_stride <= KV4_SEG_PAGES) return e;  // no sequence can be split
+  // the join of split sequences, its launch overlapped with the attention
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((size_t)p.c.n_rows * p.n_head + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<HD, T, A::PAIRS>, p);
+}
+
+extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, const void* q, size_t q_stride,
+                                                uint32_t n_head, float scale, void* workspace,
+                                                size_t workspace_bytes, void* out, void* stream) {
+  Kv4AttnParams p{};
+  bool none = false;
+  foxcuda_status st = check_kv4(c, type, "kv4_attention", &p.c, &none);
+  if (st) return st;
+  const uint32_t gqa = n_head / c->n_head_kv;
+  if (!n_head || n_head > 1024 || n_head % c->n_head_kv || (gqa != 1 && gqa != 2 && gqa != 4 && gqa != 8))
+    return fail(FOXCUDA_ERR_UNSUPPORTED, "kv4_attention: %u heads over %u KV heads are not covered", n_head, c->n_head_kv);
+  if (!(scale >= 0.0f) || scale > 3.0e38f) return fail(FOXCUDA_ERR_ARG, "kv4_attention: scale %g", (double)scale);
+  if (none) return FOXCUDA_OK;
+  if (!q || !out || !workspace) return fail(FOXCUDA_ERR_ARG, "kv4_attention: null pointer");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) ||
+      !stride_ok(q_stride, (size_t)n_head * c->head_dim, type))
+    return fail(FOXCUDA_ERR_ARG, "kv4_attention: rows and workspace must be 16-byte aligned, rows at least a row apart");
+  const size_t need = foxcuda_kv4_attention_workspace(c->n_seq, c->n_rows, n_head, c->head_dim);
+  if (workspace_bytes < need)
+    return fail(FOXCUDA_ERR_ARG, "kv4_attention: the workspace holds %zu bytes, %zu are needed", workspace_bytes, need);
+  p.q = q; p.out = out; p.part = static_cast<float*>(workspace); p.q_stride = q_stride;
+  p.n_head = (int)n_head; p.sms = current_sms();
+  p.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim);
+  CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
+       return launch_kv4_attend<decltype(tag), hd.value, 1>(p, (cudaStream_t)stream);
+     }), "kv4_attention launch");
+  return FOXCUDA_OK;
+}
