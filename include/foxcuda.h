@@ -226,13 +226,12 @@ foxcuda_status foxcuda_kv4_read(const foxcuda_kv4 *c, int ggml_type, void *k, vo
  * are rows of n_head * head_dim FOXCUDA_F32 or FOXCUDA_F16 values, q's
  * q_stride elements apart. n_head / n_head_kv is 1, 2, 4 or 8; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). The sums and softmax
- * statistics are fp32, with fp16 queries the softmax weights are rounded to
- * fp16. A row's result depends on its own sequence's lengths, not on the
- * other sequences of the call. workspace holds
+ * statistics are fp32. The same call gives the same bits; a row's sums are
+ * split where an even division of the call's pages falls, so its last bits
+ * can differ beside other sequences. workspace holds
  * foxcuda_kv4_attention_workspace() bytes (16-byte aligned; need not be
- * initialised); calls that may run at the same time must not share it. */
-size_t         foxcuda_kv4_attention_workspace(uint32_t n_seq, uint32_t n_rows, uint32_t n_head,
-                                               uint32_t head_dim);
+ * initialised) of the current device; calls that may run at the same time must not share it. */
+size_t         foxcuda_kv4_attention_workspace(uint32_t head_dim);
 foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4 *c, int ggml_type, const void *q, size_t q_stride,
                                      uint32_t n_head, float scale, void *workspace,
                                      size_t workspace_bytes, void *out, void *stream);

@@ -87,7 +87,7 @@ _PROTOS = {
     "foxcuda_kv4_block_bytes": (_sz, [C.c_uint32]),
     "foxcuda_kv4_write": (_st, [_vp, C.c_int, _vp, _sz, _vp, _sz, _vp]),
     "foxcuda_kv4_read": (_st, [_vp, C.c_int, _vp, _vp, _vp]),
-    "foxcuda_kv4_attention_workspace": (_sz, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "foxcuda_kv4_attention_workspace": (_sz, [C.c_uint32]),
     "foxcuda_kv4_attention": (_st, [_vp, C.c_int, _vp, _sz, C.c_uint32, C.c_float, _vp, _sz, _vp, _vp]),
     "foxcuda_qk_norm_rope": (_st, [C.c_int, _vp, _sz, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
                                    _vp, _vp, C.c_float, _vp, _vp, C.c_uint32, C.c_int, _vp, _vp, _sz,
@@ -485,7 +485,7 @@ def kv4_attention(q, cache, table, row_start, kv_len, scale: float = 0.0, out=No
     L = lib()
     d = _same_device(what, cache, table, row_start, kv_len, q, out, workspace)
     if workspace is None:
-        workspace = torch.empty(kv4_attention_workspace(c.n_seq, n, heads, c.head_dim, d), dtype=torch.uint8,
+        workspace = torch.empty(kv4_attention_workspace(c.head_dim, d), dtype=torch.uint8,
                                 device=q.device)
     elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
         _bad(what, "workspace is a contiguous uint8 tensor")
@@ -494,13 +494,13 @@ def kv4_attention(q, cache, table, row_start, kv_len, scale: float = 0.0, out=No
     return out
 
 
-def kv4_attention_workspace(n_seq: int, n_rows: int, n_head: int, head_dim: int, device: int | None = None) -> int:
+def kv4_attention_workspace(head_dim: int, device: int | None = None) -> int:
     """Bytes of kv4_attention's workspace (on `device`, or the current one)."""
     import torch
     if device is None or device == torch.cuda.current_device():
-        return lib().foxcuda_kv4_attention_workspace(n_seq, n_rows, n_head, head_dim)
+        return lib().foxcuda_kv4_attention_workspace(head_dim)
     with torch.cuda.device(device):
-        return lib().foxcuda_kv4_attention_workspace(n_seq, n_rows, n_head, head_dim)
+        return lib().foxcuda_kv4_attention_workspace(head_dim)
 
 
 def qk_norm_rope(x, n_head: int, n_head_kv: int, head_dim: int, pos, cos, sin, q_norm=None, k_norm=None,

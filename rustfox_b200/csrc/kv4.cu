@@ -1,5 +1,6 @@
 // The 4-bit paged K/V cache's entry points (include/foxcuda.h): argument
 // checks and launches of kv4.cuh and kv4_attn.cuh.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -130,33 +131,48 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
   return FOXCUDA_OK;
 }
 
-extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t n_seq, uint32_t n_rows, uint32_t n_head, uint32_t head_dim) {
-  if (!n_head || !kv4_hd_ok(head_dim)) return 0;
-  const size_t extra = (size_t)kv4_extra_slots((int)n_head, 8, current_sms());
-  return ((size_t)n_rows + n_seq * extra) * n_head * (head_dim + 4) * 4;
+// Two partial results of a tile for every worker.
+template <int HD, int NT>
+static size_t kv4_part_bytes(int ctas) {
+  using A = Kv4Attn<HD, NT>;
+  return (size_t)ctas * A::NW * 2 * A::PAIRS * A::PART * 4;
+}
+
+extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim) {
+  const int ctas = current_sms();
+  switch (head_dim) {
+    case 64: return kv4_part_bytes<64, 1>(ctas);
+    case 128: return kv4_part_bytes<128, 1>(ctas);
+    case 256: return kv4_part_bytes<256, 1>(ctas);
+    default: return 0;
+  }
 }
 
 template <typename T, int HD, int NT>
 static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
   using A = Kv4Attn<HD, NT>;
   const size_t smem = A::smem_bytes(p.c.n_seq);
-  static size_t marks[kMaxDevices] = {};
+  static size_t marks[kMaxDevices] = {}, join_marks[kMaxDevices] = {};
   cudaError_t e = opt_in_smem(kv4_attend_kernel<HD, T, NT>, smem, marks);
   if (e != cudaSuccess) return e;
-  kv4_attend_kernel<HD, T, NT><<<p.sms, A::NW * 32, smem, s>>>(p);
+  kv4_attend_kernel<HD, T, NT><<<p.ctas, A::NW * 32, smem, s>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if (p.c.table_stride <= KV4_SEG_PAGES) return e;  // no sequence can be split
-  // the join of split sequences, its launch overlapped with the attention
+  if (p.c.table_stride <= KV4_MIN_PAGES) return e;  // no run can be split
+  // the join of split runs, its launch overlapped with the attention
+  const int gqa = p.n_head / p.c.n_kv;
+  const size_t most = ((size_t)p.c.n_rows * gqa / A::PAIRS + p.c.n_seq) * p.c.n_kv * A::PAIRS;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(((size_t)p.c.n_rows * p.n_head + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)std::min<size_t>(most, (size_t)p.ctas * 4));
+  cfg.blockDim = dim3(KV4_JOIN_WARPS * 32);
+  cfg.dynamicSmemBytes = (KV4_JOIN_WARPS * (HD + 1) + KV4_JOIN_WARPS) * 4 + (size_t)(p.c.n_seq + 1) * 16;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<HD, T, A::PAIRS>, p);
+  if ((e = opt_in_smem(kv4_join_kernel<HD, T, NT>, cfg.dynamicSmemBytes, join_marks)) != cudaSuccess) return e;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, NT>, p);
 }
 
 extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, const void* q, size_t q_stride,
@@ -175,11 +191,11 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) ||
       !stride_ok(q_stride, (size_t)n_head * c->head_dim, type))
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: rows and workspace must be 16-byte aligned, rows at least a row apart");
-  const size_t need = foxcuda_kv4_attention_workspace(c->n_seq, c->n_rows, n_head, c->head_dim);
+  const size_t need = foxcuda_kv4_attention_workspace(c->head_dim);
   if (workspace_bytes < need)
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: the workspace holds %zu bytes, %zu are needed", workspace_bytes, need);
   p.q = q; p.out = out; p.part = static_cast<float*>(workspace); p.q_stride = q_stride;
-  p.n_head = (int)n_head; p.sms = current_sms();
+  p.n_head = (int)n_head; p.ctas = current_sms();
   p.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim);
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
        return launch_kv4_attend<decltype(tag), hd.value, 1>(p, (cudaStream_t)stream);

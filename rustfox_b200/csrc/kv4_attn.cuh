@@ -27,8 +27,7 @@
 //   and a negated weight: the second product's sums then stay near the result
 //   instead of 7.5 d away from it. They round toward zero, so what would
 //   cancel in the end must not pass through them: at 32768 positions the error
-//   was 1e-4 of the result with all positions counted from below. A page's
-//   sums start at zero and join the rest in plain fp32 for the same reason.
+//   was 1e-4 of the result with all positions counted from below.
 #pragma once
 
 #include <climits>
@@ -43,36 +42,97 @@ struct Kv4AttnParams {
   Kv4Rows c;
   const void* q;
   void* out;
-  float* part;       // partial results of split sequences
+  float* part;       // partial results of split runs, two a worker
   size_t q_stride;   // elements between rows
-  int n_head, sms;
+  int n_head, ctas;
   float scale;
 };
 
-// How a sequence of L positions and T rows is cut, from its own numbers and
-// the device's: tiles of `pairs` (row, head) pairs of a KV head, and segments
-// of pages that different CTAs take when rows and heads alone do not fill the
-// device.
-constexpr int KV4_SEG_PAGES = 4;    // pages a segment has at least
-struct Kv4Cut { int tiles, segs; };
-__host__ __device__ inline Kv4Cut kv4_cut(int L, int T, int gqa, int n_kv, int pairs, int sms) {
-  Kv4Cut k;
-  k.tiles = (T * gqa + pairs - 1) / pairs;
-  const int pages = (L + KV_PAGE - 1) / KV_PAGE;
-  const int want = sms / max(1, n_kv * k.tiles), most = (pages + KV4_SEG_PAGES - 1) / KV4_SEG_PAGES;
-  k.segs = max(1, min(want, most));
-  return k;
+// How the work is divided. A tile is PAIRS (row, head) pairs of one KV head of
+// a sequence, a run all the pages of its sequence, and a warp is a worker:
+// the runs stand in a line (sequence, tile, KV head), and every worker takes
+// an equal stretch of the line's pages. A worker that holds a whole run writes
+// its result; the pieces of a split one go to the workspace (a worker holds at
+// most two: the end of one run and the beginning of another) and are joined in
+// order by a second kernel. So the load is even whatever the lengths, and no
+// worker waits for another.
+constexpr int KV4_MIN_PAGES = 1;  // pages a worker takes at least
+struct Kv4Line {
+  long long* page0;  // [n_seq + 1] first page in line of each sequence
+  long long* run0;   // [n_seq + 1] first run of each sequence
+};
+struct Kv4Seq { int r0, T, L, tiles, pages; };
+
+template <int PAIRS>
+FOX_DEV Kv4Seq kv4_seq(const Kv4AttnParams& p, int s) {
+  Kv4Seq q;
+  q.r0 = min(max(__ldg(p.c.row_start + s), 0), p.c.n_rows);
+  q.T = min(max(__ldg(p.c.row_start + s + 1), q.r0), p.c.n_rows) - q.r0;
+  q.L = kv4_len(p.c, s);
+  q.tiles = (q.T * (p.n_head / p.c.n_kv) + PAIRS - 1) / PAIRS;
+  q.pages = max(1, (q.L + KV_PAGE - 1) / KV_PAGE);  // one even where nothing is cached: its rows get zeros
+  return q;
 }
-// Slots of partial results a sequence can need beyond one for each row.
-__host__ __device__ inline int kv4_extra_slots(int n_head, int pairs, int sms) {
-  return (sms * pairs + n_head - 1) / n_head;
+
+// Prefix sums of the sequences' runs and pages, by the CTA's first warp.
+template <int PAIRS>
+FOX_DEV void kv4_line(const Kv4AttnParams& p, const Kv4Line& line) {
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    long long runs = 0, pages = 0;
+    for (int s0 = 0; s0 < p.c.n_seq; s0 += 32) {
+      const int s = s0 + lane;
+      long long r = 0, n = 0;
+      if (s < p.c.n_seq) {
+        const Kv4Seq q = kv4_seq<PAIRS>(p, s);
+        r = (long long)q.tiles * p.c.n_kv;
+        n = r * q.pages;
+      }
+      long long rs = r, ns = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long ru = __shfl_up_sync(0xffffffffu, rs, o), nu = __shfl_up_sync(0xffffffffu, ns, o);
+        if (lane >= o) { rs += ru; ns += nu; }
+      }
+      if (s < p.c.n_seq) { line.run0[s] = runs + rs - r; line.page0[s] = pages + ns - n; }
+      runs += __shfl_sync(0xffffffffu, rs, 31);
+      pages += __shfl_sync(0xffffffffu, ns, 31);
+    }
+    if (lane == 0) { line.run0[p.c.n_seq] = runs; line.page0[p.c.n_seq] = pages; }
+  }
+  __syncthreads();
 }
+
+// The last sequence that begins at or before x (sequences without runs take
+// no room, so it is the one that holds x).
+FOX_DEV int kv4_find(const long long* start, int n_seq, long long x) {
+  int lo = 0, hi = n_seq - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (start[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Worker w of W takes pages w * U / W .. (w + 1) * U / W - 1 of the line's U.
+FOX_DEV int kv4_workers(long long U, int ctas, int nw) {
+  return (int)min((long long)ctas * nw, (U + KV4_MIN_PAGES - 1) / KV4_MIN_PAGES);
+}
+FOX_DEV long long kv4_first(long long w, long long U, int W) { return w * U / W; }
+FOX_DEV int kv4_owner(long long u, long long U, int W) { return (int)(((u + 1) * W - 1) / U); }
 
 FOX_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from zero.
+FOX_DEV void mma16816_0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 FOX_DEV uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -99,17 +159,25 @@ FOX_DEV void kv4_operands(uint32_t x, uint32_t (&a)[4]) {
   a[3] = (down & O) ^ FO;
 }
 constexpr float KV4_EVEN = 4194304.0f;  // 2^22
+// A weight may exceed 1 by 2^SLACK before the sums are rescaled; times d it is
+// scaled to at most 2^15.
+constexpr float KV4_SLACK = 7.0f, KV4_WEIGHT = 256.0f;
 // x as hi + lo fp16: hi keeps the leading 11 bits.
 FOX_DEV uint32_t kv4_hi_lo(float x) {
   const float hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
   return half2_bits(__floats2half2_rn(hi, x - hi));
 }
 
-// What a warp's pages are: a range of pages of one sequence and KV head.
-struct Kv4Item {
-  int seq, kv, tile, seg, segs, first, last;  // pages first .. last-1
-  int r0, T, L;
+// A page in line: page `page` of a run.
+struct Kv4Unit {
+  Kv4Seq q;
+  int seq, tile, kv, page;
 };
+
+FOX_DEV float4 kv4_quotient(float4 v, float l) {
+  if (l == 0.0f) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // nothing to see
+  return make_float4(__fdiv_rn(v.x, l), __fdiv_rn(v.y, l), __fdiv_rn(v.z, l), __fdiv_rn(v.w, l));
+}
 
 // HD: head dimension; NT: column tiles (of 4 pairs) of a warp.
 template <int HD, int NT>
@@ -117,13 +185,11 @@ struct Kv4Attn {
   static constexpr int SLAB = HD < 128 ? HD : 128, SLABS = HD / SLAB, SG = SLAB / 64, NB = SLAB / 32;
   static constexpr int G = HD / KV4_GROUP, BB = kv4_block_bytes(HD), PAGE_BYTES = 2 * BB;
   static constexpr int PAIRS = 4 * NT;       // (row, head) pairs of a tile
-  static constexpr int RED_STRIDE = HD + 4;  // floats of one pair of one warp
-  // warps of a CTA and pages in flight per warp: what shared memory holds
-  static constexpr int NW = HD == 64 ? 12 : HD == 128 ? 10 : 5, SLOTS = HD == 64 ? 3 : 2;
-  static constexpr size_t ring_bytes() { return (size_t)NW * SLOTS * PAGE_BYTES; }
-  static constexpr size_t red_bytes() { return (size_t)NW * PAIRS * RED_STRIDE * 4; }
+  static constexpr int PART = HD + 4;        // floats of one pair's partial result: M, l, -, -, sums
+  // warps of a CTA, each with room for a page's K and V: what the registers hold
+  static constexpr int NW = HD < 256 ? 12 : 8;
   static constexpr size_t smem_bytes(int n_seq) {
-    return ring_bytes() + red_bytes() + NW * PAIRS * 8 + NW * SLOTS * 8 + (size_t)(n_seq + 1) * 4 + 16;
+    return (size_t)NW * PAGE_BYTES + NW * 2 * 8 + (size_t)(n_seq + 1) * 16;
   }
 
   // A warp's share of a tile: q's operand registers, and the running maximum,
@@ -133,28 +199,30 @@ struct Kv4Attn {
   uint32_t qb[NT][SLABS][SG][2][2][2];
   float f[NT], qs[NT][G];  // score = f * sum_g (d_g * product) + sum_g m_g * qs_g, in powers of 2
   float o[NT][SLABS][NB][2][4], mx[NT], l[NT], mo[NT][G], big;
+  float sco[NT][4][2];            // the page's scores
   int lim[NT], lim_min, lim_max;  // the last position a pair sees (negative: none; no pair: all), and over the tile
 
-  FOX_DEV void limits(const Kv4Item& it, int gqa) {
-    const int t = threadIdx.x & 3;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int pr = it.tile * PAIRS + n * 4 + t;
-      lim[n] = pr < it.T * gqa ? it.L - it.T + pr / gqa : INT_MAX;
-    }
-    lim_min = max(0, it.L - it.T + it.tile * PAIRS / gqa);
-    lim_max = it.L - it.T + min(it.T - 1, (it.tile * PAIRS + PAIRS - 1) / gqa);
+  // The last position that any row of a tile sees.
+  static FOX_DEV int last_seen(const Kv4Seq& q, int tile, int gqa) {
+    return q.L - q.T + min(q.T - 1, (tile * PAIRS + PAIRS - 1) / gqa);
   }
 
   template <typename T>
-  FOX_DEV void load_q(const Kv4AttnParams& p, const Kv4Item& it, int gqa) {
+  FOX_DEV void begin(const Kv4AttnParams& p, const Kv4Unit& it, int gqa) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int pr = it.tile * PAIRS + n * 4 + t;
+      lim[n] = pr < it.q.T * gqa ? it.q.L - it.q.T + pr / gqa : INT_MAX;
+    }
+    lim_min = max(0, it.q.L - it.q.T + it.tile * PAIRS / gqa);
+    lim_max = last_seen(it.q, it.tile, gqa);
     const float unit = p.scale * 1.44269504088896341f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int pr = it.tile * PAIRS + n * 4 + (g >> 1);
-      const bool live = pr < it.T * gqa;
-      const int row = it.r0 + (live ? pr / gqa : 0), head = it.kv * gqa + (live ? pr % gqa : 0);
+      const bool live = pr < it.q.T * gqa;
+      const int row = it.q.r0 + (live ? pr / gqa : 0), head = it.kv * gqa + (live ? pr % gqa : 0);
       const T* q = static_cast<const T*>(p.q) + (size_t)row * p.q_stride + (size_t)head * HD;
       float x[G][16], top = 0.0f, sum[G];
 #pragma unroll
@@ -212,15 +280,10 @@ struct Kv4Attn {
     big = 0x1p-24f;  // a power of two above every d met
   }
 
-  // One page in shared memory. EDGE: some of its positions are hidden from
-  // some pair (`absent`: all of them from all).
-  template <bool EDGE>
-  FOX_DEV void page(const uint8_t* kb, int pos0, bool absent) {
+  // The scores of a page's K block.
+  FOX_DEV void scores(const uint8_t* kb) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint8_t* vb = kb + BB;
-    const __half2* kdm = reinterpret_cast<const __half2*>(kb + kv4_codes_bytes(HD));
-    const __half2* vdm = reinterpret_cast<const __half2*>(vb + kv4_codes_bytes(HD));
-    float sco[NT][4][2];
+    const __half2* dm = reinterpret_cast<const __half2*>(kb + kv4_codes_bytes(HD));
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int a = s * 16 + g;
@@ -239,7 +302,7 @@ struct Kv4Attn {
 #pragma unroll
         for (int j = 0; j < SG; ++j) {
           const int gg = sl * SG + j;
-          float c[NT][4] = {};
+          float c[NT][4];
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             uint32_t x[4], y[4];
@@ -247,11 +310,13 @@ struct Kv4Attn {
             kv4_operands<false>(wb[2 * j + w], y);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma16816(c[n], x[0], y[0], x[1], y[1], qb[n][sl][j][w][0][0], qb[n][sl][j][w][0][1]);
-              mma16816(c[n], x[2], y[2], x[3], y[3], qb[n][sl][j][w][1][0], qb[n][sl][j][w][1][1]);
+              const uint32_t(&b)[2][2] = qb[n][sl][j][w];
+              if (w == 0) mma16816_0(c[n], x[0], y[0], x[1], y[1], b[0][0], b[0][1]);
+              else mma16816(c[n], x[0], y[0], x[1], y[1], b[0][0], b[0][1]);
+              mma16816(c[n], x[2], y[2], x[3], y[3], b[1][0], b[1][1]);
             }
           }
-          const float2 da = __half22float2(kdm[a * G + gg]), db = __half22float2(kdm[(a + 8) * G + gg]);
+          const float2 da = __half22float2(dm[a * G + gg]), db = __half22float2(dm[(a + 8) * G + gg]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const float ca = c[n][0] + c[n][1], cb = c[n][2] + c[n][3];
@@ -267,40 +332,47 @@ struct Kv4Attn {
 #pragma unroll
         for (int h = 0; h < 2; ++h) sco[n][s][h] = fmaf(prod[n][h], f[n], off[n][h]);
     }
+  }
 
-    // V's parameters of this lane's positions, the page's largest d, and the
-    // maxima over its positions
-    float2 dv[4][2][G];
-    float dmax = 0.0f, top[NT];
-    const float from_top = (g & 1) ? 15.0f : 0.0f;
+  // Softmax weights of the page's scores and the sums over its V block. EDGE:
+  // some of its positions are hidden from some pair.
+  template <bool EDGE>
+  FOX_DEV void values(const uint8_t* vb, int pos0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const __half2* dm = reinterpret_cast<const __half2*>(vb + kv4_codes_bytes(HD));
+    // this lane's parameters, the page's largest d, the maxima over its positions
+    __half2 dv[4][2][G], most = __half2half2(__ushort_as_half(0));
+    float top[NT];
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = s * 16 + h * 8 + g;
-        const bool nobody = EDGE && (absent || pos0 + at > lim_max);
+        const bool nobody = EDGE && pos0 + at > lim_max;
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-          dv[s][h][j] = __half22float2(vdm[at * G + j]);
-          if (nobody) dv[s][h][j] = make_float2(0.0f, 0.0f);  // whatever the memory held
-          dmax = fmaxf(dmax, dv[s][h][j].x);
-          dv[s][h][j].y = fmaf(from_top, dv[s][h][j].x, dv[s][h][j].y);
+          dv[s][h][j] = dm[at * G + j];
+          if (nobody) dv[s][h][j] = __half2half2(__ushort_as_half(0));  // whatever the memory held
+          most = __hmax2(most, dv[s][h][j]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          if (EDGE && (absent || pos0 + at > lim[n])) sco[n][s][h] = -INFINITY;
+          if (EDGE && pos0 + at > lim[n]) sco[n][s][h] = -INFINITY;
           top[n] = s + h ? fmaxf(top[n], sco[n][s][h]) : sco[n][s][h];
         }
       }
 #pragma unroll
     for (int sh = 4; sh < 32; sh <<= 1) {
-      dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, sh));
+      most = __hmax2(most, __shfl_xor_sync(0xffffffffu, most, sh));
 #pragma unroll
       for (int n = 0; n < NT; ++n) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], sh));
     }
+    const float dmax = __low2float(most);
+    // The reference point of a pair's weights moves only when a score passes
+    // it by 2^KV4_SLACK: the weights' scale leaves room for that.
     bool grew = dmax >= big;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) grew = grew || top[n] > mx[n];
+    for (int n = 0; n < NT; ++n) grew = grew || top[n] > mx[n] + KV4_SLACK;
     if (__any_sync(0xffffffffu, grew)) {
       const float to = dmax >= big ? __uint_as_float((__float_as_uint(dmax) & 0x7f800000u) + 0x00800000u) : big;
       const float shrink = big / to;
@@ -325,70 +397,64 @@ struct Kv4Attn {
     }
 
     // the weights, times d, as the second product's operand
-    const float norm = ((g & 1) ? -32768.0f : 32768.0f) / big;
-    uint32_t pb[NT][4][G][2];
+    const float norm = ((g & 1) ? -KV4_WEIGHT : KV4_WEIGHT) / big, from_top = (g & 1) ? 15.0f : 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float base = EDGE && mx[n] == -INFINITY ? 0.0f : mx[n];
+    for (int s = 0; s < 4; ++s) {
+      uint32_t pb[NT][G][2];
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+      for (int h = 0; h < 2; ++h) {
+        float w[NT], wn[NT];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float w = exp2_approx(sco[n][s][h] - base), wn = w * norm;
-          l[n] += w;
-#pragma unroll
-          for (int j = 0; j < G; ++j) {
-            float v = wn * dv[s][h][j].x, m = dv[s][h][j].y;
-            if (EDGE && sco[n][s][h] == -INFINITY) v = m = 0.0f;  // hidden, whatever it is
-            mo[n][j] = fmaf(w, m, mo[n][j]);
-            pb[n][s][j][h] = transpose8x8(kv4_hi_lo(v));
-          }
+        for (int n = 0; n < NT; ++n) {
+          w[n] = exp2_approx(sco[n][s][h] - (EDGE && mx[n] == -INFINITY ? 0.0f : mx[n]));
+          wn[n] = w[n] * norm;
+          l[n] += w[n];
         }
-    }
 #pragma unroll
-    for (int sl = 0; sl < SLABS; ++sl) {
-      uint32_t u[4][NB], v[4][NB];
+        for (int j = 0; j < G; ++j) {
+          const float2 d = __half22float2(dv[s][h][j]);
+          const float m = fmaf(from_top, d.x, d.y);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const uint8_t* base = vb + ((((sl * 4 + s) * 2) * 4 + t) * 8 + g) * (4 * NB);
-        if constexpr (NB == 4) {
-          *reinterpret_cast<uint4*>(u[s]) = *reinterpret_cast<const uint4*>(base);
-          *reinterpret_cast<uint4*>(v[s]) = *reinterpret_cast<const uint4*>(base + 32 * 4 * NB);
-        } else {
-          *reinterpret_cast<uint2*>(u[s]) = *reinterpret_cast<const uint2*>(base);
-          *reinterpret_cast<uint2*>(v[s]) = *reinterpret_cast<const uint2*>(base + 32 * 4 * NB);
+          for (int n = 0; n < NT; ++n) {
+            const bool hidden = EDGE && sco[n][s][h] == -INFINITY;  // whatever it is
+            mo[n][j] = fmaf(w[n], hidden ? 0.0f : m, mo[n][j]);
+            pb[n][j][h] = transpose8x8(kv4_hi_lo(hidden ? 0.0f : wn[n] * d.x));
+          }
         }
       }
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int j = sl * SG + b / 2;
-        float c[NT][2][4] = {};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          uint32_t x[4], y[4];
-          kv4_operands<true>(u[s][b], x);
-          kv4_operands<true>(v[s][b], y);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma16816(c[n][0], x[0], x[1], y[0], y[1], pb[n][s][j][0], pb[n][s][j][1]);
-            mma16816(c[n][1], x[2], x[3], y[2], y[3], pb[n][s][j][0], pb[n][s][j][1]);
-          }
+      for (int sl = 0; sl < SLABS; ++sl) {
+        uint32_t u[NB], v[NB];
+        const uint8_t* base = vb + ((((sl * 4 + s) * 2) * 4 + t) * 8 + g) * (4 * NB);
+        if constexpr (NB == 4) {
+          *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(base);
+          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(base + 32 * 4 * NB);
+        } else {
+          *reinterpret_cast<uint2*>(u) = *reinterpret_cast<const uint2*>(base);
+          *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(base + 32 * 4 * NB);
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int b = 0; b < NB; ++b) {
+          const int j = sl * SG + b / 2;
+          uint32_t x[4], y[4];
+          kv4_operands<true>(u[b], x);
+          kv4_operands<true>(v[b], y);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[n][sl][b][h][i] += c[n][h][i];
+          for (int n = 0; n < NT; ++n) {
+            mma16816(o[n][sl][b][0], x[0], x[1], y[0], y[1], pb[n][j][0], pb[n][j][1]);
+            mma16816(o[n][sl][b][1], x[2], x[3], y[2], y[3], pb[n][j][0], pb[n][j][1]);
+          }
+        }
       }
     }
   }
 
-  // The warp's sums over its lanes' positions, to its part of `red` (PAIRS
-  // rows) and redm.
-  FOX_DEV void park(float* red, float2* redm) {
+  // The run's results: to `part` (PAIRS partial results), or to the rows of
+  // out where that is null.
+  template <typename T>
+  FOX_DEV void end(const Kv4AttnParams& p, const Kv4Unit& it, int gqa, float* part) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const float unit = big * (KV4_EVEN / 32768.0f);
+    const float unit = big * (KV4_EVEN / KV4_WEIGHT);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -397,217 +463,193 @@ struct Kv4Attn {
 #pragma unroll
         for (int j = 0; j < G; ++j) mo[n][j] += __shfl_xor_sync(0xffffffffu, mo[n][j], sh);
       }
-      float* dst = red + (size_t)(n * 4 + t) * RED_STRIDE;
+      const int pr = it.tile * PAIRS + n * 4 + t;
+      if (pr >= it.q.T * gqa) continue;
+      T* out = static_cast<T*>(p.out) + ((size_t)(it.q.r0 + pr / gqa) * p.n_head + it.kv * gqa + pr % gqa) * HD;
+      float* dst = part + (size_t)(n * 4 + t) * PART;
 #pragma unroll
       for (int sl = 0; sl < SLABS; ++sl)
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const float m = mo[n][sl * SG + b / 2];
           const float(&c)[2][4] = o[n][sl][b];
-          *reinterpret_cast<float4*>(dst + sl * SLAB + b * 32 + g * 4) =
-              make_float4(fmaf(c[0][0] + c[0][1], unit, m), fmaf(c[0][2] + c[0][3], unit * 0.0625f, m),
-                          fmaf(c[1][0] + c[1][1], unit, m), fmaf(c[1][2] + c[1][3], unit * 0.0625f, m));
+          float4 v = make_float4(fmaf(c[0][0] + c[0][1], unit, m), fmaf(c[0][2] + c[0][3], unit * 0.0625f, m),
+                                 fmaf(c[1][0] + c[1][1], unit, m), fmaf(c[1][2] + c[1][3], unit * 0.0625f, m));
+          const int d = sl * SLAB + b * 32 + g * 4;
+          if (part) *reinterpret_cast<float4*>(dst + 4 + d) = v;
+          else kv4_store4(out + d, kv4_quotient(v, l[n]));
         }
-      if (g == 0) redm[n * 4 + t] = make_float2(mx[n], l[n]);
+      if (part && g == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx[n], l[n]);
     }
   }
 };
 
-// Prefix sums of every sequence's items (tiles x KV heads x segments) in
-// shared memory, by the CTA's first warp.
-template <int PAIRS>
-FOX_DEV void kv4_schedule(const Kv4AttnParams& p, int* start) {
-  const int lane = threadIdx.x & 31;
-  if (threadIdx.x < 32) {
-    int base = 0;
-    for (int s0 = 0; s0 < p.c.n_seq; s0 += 32) {
-      const int s = s0 + lane;
-      int n = 0;
-      if (s < p.c.n_seq) {
-        const int a = min(max(__ldg(p.c.row_start + s), 0), p.c.n_rows);
-        const int b = min(max(__ldg(p.c.row_start + s + 1), a), p.c.n_rows);
-        if (b > a) {
-          const Kv4Cut k = kv4_cut(kv4_len(p.c, s), b - a, p.n_head / p.c.n_kv, p.c.n_kv, PAIRS, p.sms);
-          n = k.tiles * k.segs * p.c.n_kv;
-        }
-      }
-      int sum = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-      }
-      if (s < p.c.n_seq) start[s] = base + sum - n;
-      base += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (lane == 0) start[p.c.n_seq] = base;
-  }
-  __syncthreads();
-}
-
-template <int PAIRS>
-FOX_DEV Kv4Item kv4_item(const Kv4AttnParams& p, const int* start, int item) {
-  int lo = 0, hi = p.c.n_seq - 1;  // the last sequence that starts at or before the item
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (start[mid] <= item) lo = mid; else hi = mid - 1;
-  }
-  Kv4Item it;
-  it.seq = lo;
-  it.r0 = min(max(__ldg(p.c.row_start + lo), 0), p.c.n_rows);
-  it.T = min(max(__ldg(p.c.row_start + lo + 1), it.r0), p.c.n_rows) - it.r0;
-  it.L = min(max(__ldg(p.c.kv_len + lo), 0), p.c.table_stride * KV_PAGE);
-  const Kv4Cut k = kv4_cut(it.L, it.T, p.n_head / p.c.n_kv, p.c.n_kv, PAIRS, p.sms);
-  int r = item - start[lo];
-  it.segs = k.segs;
-  it.seg = r % k.segs; r /= k.segs;
-  it.kv = r % p.c.n_kv;
-  it.tile = r / p.c.n_kv;
-  const int pages = (it.L + KV_PAGE - 1) / KV_PAGE;
-  it.first = (int)((long long)pages * it.seg / k.segs);
-  it.last = (int)((long long)pages * (it.seg + 1) / k.segs);
-  return it;
-}
-
 template <int HD, typename T, int NT>
 __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel(const Kv4AttnParams p) {
   using A = Kv4Attn<HD, NT>;
-  constexpr int PAIRS = A::PAIRS, NW = A::NW, SLOTS = A::SLOTS;
+  constexpr int PAIRS = A::PAIRS, NW = A::NW;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem + A::ring_bytes());
-  float2* redm = reinterpret_cast<float2*>(smem + A::ring_bytes() + A::red_bytes());  // (M, l) of a warp's pair
-  uint64_t* bars = reinterpret_cast<uint64_t*>(redm + NW * PAIRS);
-  int* start = reinterpret_cast<int*>(bars + NW * SLOTS);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint8_t* ring = smem + (size_t)warp * SLOTS * A::PAGE_BYTES;
-  uint64_t* bar = bars + warp * SLOTS;
+  uint8_t* ring = smem + (size_t)warp * A::PAGE_BYTES;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + (size_t)NW * A::PAGE_BYTES) + warp * 2;
+  Kv4Line line;
+  line.page0 = reinterpret_cast<long long*>(smem + (size_t)NW * A::PAGE_BYTES + NW * 2 * 8);
+  line.run0 = line.page0 + p.c.n_seq + 1;
   const int gqa = p.n_head / p.c.n_kv;
 
   if (lane == 0) {
-    for (int i = 0; i < SLOTS; ++i) mbar_init(bar + i, 1);
+    mbar_init(bar, 1);
+    mbar_init(bar + 1, 1);
     mbar_fence_init();
   }
   __syncwarp();
   griddep_wait();
   griddep_launch_dependents();
-  kv4_schedule<PAIRS>(p, start);
-  const int n_items = start[p.c.n_seq];
+  kv4_line<PAIRS>(p, line);
+  const long long U = line.page0[p.c.n_seq];
+  if (U == 0) return;
+  // neighbours in line sit on different SMs
+  const int W = kv4_workers(U, gridDim.x, NW), worker = warp * gridDim.x + blockIdx.x;
+  if (worker >= W) return;
+  const long long u0 = kv4_first(worker, U, W), u1 = kv4_first(worker + 1, U, W);
+
+  auto locate = [&](long long u) {
+    Kv4Unit x;
+    x.seq = kv4_find(line.page0, p.c.n_seq, u);
+    x.q = kv4_seq<PAIRS>(p, x.seq);
+    const long long at = u - line.page0[x.seq], run = at / x.q.pages;
+    x.page = (int)(at - run * x.q.pages);
+    x.kv = (int)(run % p.c.n_kv);
+    x.tile = (int)(run / p.c.n_kv);
+    return x;
+  };
+  // The page's K block, or null where there is nothing to see: no row of the
+  // tile reaches it, or the table names no page there.
+  auto find = [&](const Kv4Unit& x) -> const uint8_t* {
+    if (x.page * KV_PAGE > A::last_seen(x.q, x.tile, gqa)) return nullptr;
+    const int page = kv4_page(p.c, x.seq, x.page * KV_PAGE);
+    return page < 0 ? nullptr : kv4_block(p.c, page, x.kv, 0, A::BB);
+  };
+  auto ask = [&](const uint8_t* block, int side) {  // the ring's K or V
+    if (block && lane == 0) {
+      mbar_arrive_expect_tx(bar + side, A::BB);
+      bulk_g2s(ring + side * A::BB, block + side * A::BB, A::BB, bar + side);
+    }
+  };
+  unsigned phase = 0;  // of both barriers
+  bool dead = false;   // a wait gave up: the results are not valid, and nothing more is asked for
+  auto arrived = [&](int side) {
+    if (__any_sync(0xffffffffu, !mbar_wait(bar + side, phase))) {
+      if (lane == 0 && p.c.err) atomicExch(p.c.err, KERR_WAIT);
+      dead = true;
+    }
+  };
 
   A w;
-  Kv4Item it;
-  int issued = 0, taken = 0;  // pages this warp asked for and used, over all items
-  int n_mine = 0;             // pages of the item this warp takes: first + warp, + NW, ...
-  bool dead = false;          // a wait gave up: nothing more is asked for
-  auto issue = [&](int i) {   // this warp's i-th page of the item
-    if (lane == 0) {
-      const int slot = issued % SLOTS;
-      const int page = kv4_page(p.c, it.seq, (it.first + warp + i * NW) * KV_PAGE);
-      // an absent page is not read: its positions are masked when taken
-      mbar_arrive_expect_tx(bar + slot, page >= 0 ? A::PAGE_BYTES : 0);
-      if (page >= 0)
-        bulk_g2s(ring + (size_t)slot * A::PAGE_BYTES, kv4_block(p.c, page, it.kv, 0, A::BB), A::PAGE_BYTES, bar + slot);
-    }
-    ++issued;
-  };
-  auto begin = [&](int item) {
-    it = kv4_item<PAIRS>(p, start, item);
-    w.limits(it, gqa);
-    const int last = min(it.last, w.lim_max < 0 ? 0 : w.lim_max / KV_PAGE + 1);
-    n_mine = last > it.first + warp ? (last - it.first - warp + NW - 1) / NW : 0;
-    for (int i = 0; i < min(n_mine, SLOTS) && !dead; ++i) issue(i);
-  };
-  if ((int)blockIdx.x < n_items) begin(blockIdx.x);
-  for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-    w.template load_q<T>(p, it, gqa);
-    for (int i = 0; i < n_mine && !dead; ++i) {
-      const int slot = taken % SLOTS, pos0 = (it.first + warp + i * NW) * KV_PAGE;
-      const int page = __ldg(p.c.table + (size_t)it.seq * p.c.table_stride + pos0 / KV_PAGE);
-      const bool absent = (unsigned)page >= (unsigned)p.c.n_pages;
-      dead = __any_sync(0xffffffffu, !mbar_wait(bar + slot, (taken / SLOTS) & 1));
-      if (dead) {
-        if (lane == 0 && p.c.err) atomicExch(p.c.err, KERR_WAIT);
-        break;
+  Kv4Unit cur = locate(u0);
+  const uint8_t* block = find(cur);
+  ask(block, 0);
+  ask(block, 1);
+  w.template begin<T>(p, cur, gqa);
+  for (long long u = u0; u < u1; ++u) {
+    // the next page: its address is known before this one's codes are used up
+    Kv4Unit nxt = cur;
+    const bool last = u + 1 == u1;
+    if (++nxt.page == nxt.q.pages && !last) nxt = locate(u + 1);
+    const uint8_t* after = last || dead ? nullptr : find(nxt);
+    if (block) {
+      const int pos0 = cur.page * KV_PAGE;
+      arrived(0);
+      if (!dead) w.scores(ring);
+      __syncwarp();  // every lane has read K
+      if (!dead) ask(after, 0);
+      arrived(1);
+      if (!dead) {
+        if (pos0 + KV_PAGE - 1 > w.lim_min) w.template values<true>(ring + A::BB, pos0);
+        else w.template values<false>(ring + A::BB, pos0);
       }
-      ++taken;
-      const uint8_t* kb = ring + (size_t)slot * A::PAGE_BYTES;
-      if (absent || pos0 + KV_PAGE - 1 > w.lim_min) w.template page<true>(kb, pos0, absent);
-      else w.template page<false>(kb, pos0, false);
-      __syncwarp();  // every lane has read the slot
-      if (i + SLOTS < n_mine) issue(i + SLOTS);
+      __syncwarp();
+      if (!dead) ask(after, 1);
+      phase ^= 1;
+    } else {
+      ask(after, 0);
+      ask(after, 1);
     }
-    w.park(red + (size_t)warp * PAIRS * A::RED_STRIDE, redm + warp * PAIRS);
-    const Kv4Item was = it;
-    // the next item's pages are on their way while this one's warps are joined
-    if (item + (int)gridDim.x < n_items) begin(item + gridDim.x);
-    __syncthreads();
-    for (int u = threadIdx.x; u < PAIRS * HD; u += NW * 32) {
-      const int pr = u / HD, d = u % HD, pair = was.tile * PAIRS + pr;
-      if (pair >= was.T * gqa) break;
-      float M = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < NW; ++k) M = fmaxf(M, redm[k * PAIRS + pr].x);
-      float sum = 0.0f, ls = 0.0f;
-#pragma unroll
-      for (int k = 0; k < NW; ++k) {
-        const float2 ml = redm[k * PAIRS + pr];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // nothing seen by this warp
-        const float by = exp2_approx(ml.x - M);
-        ls = fmaf(ml.y, by, ls);
-        sum = fmaf(red[(size_t)(k * PAIRS + pr) * A::RED_STRIDE + d], by, sum);
-      }
-      const int row = pair / gqa, head = was.kv * gqa + pair % gqa;
-      if (was.segs == 1) {
-        const float r = ls == 0.0f ? 0.0f : __fdiv_rn(sum, ls);  // nothing to see: zeros
-        static_cast<T*>(p.out)[((size_t)(was.r0 + row) * p.n_head + head) * HD + d] = (T)r;
-      } else {
-        const size_t slot = (size_t)was.r0 + (size_t)was.seq * kv4_extra_slots(p.n_head, PAIRS, p.sms) +
-                            (size_t)row * was.segs + was.seg;
-        float* dst = p.part + (slot * p.n_head + head) * (HD + 4);
-        dst[4 + d] = sum;
-        if (d == 0) { dst[0] = M; dst[1] = ls; }
-      }
+    if (last || nxt.page == 0 || nxt.page == nxt.q.pages) {  // the run's end, or this worker's
+      const long long run_first = u - cur.page;
+      const bool whole = run_first >= u0 && cur.page + 1 == cur.q.pages;
+      float* part = p.part + ((size_t)worker * 2 + (run_first <= u0 ? 0 : 1)) * (PAIRS * A::PART);
+      w.template end<T>(p, cur, gqa, whole ? nullptr : part);
+      if (!last) w.template begin<T>(p, nxt, gqa);
     }
-    __syncthreads();  // red is free
+    cur = nxt;
+    block = dead ? nullptr : after;
   }
-  // copies in flight end before the CTA does
-  for (; taken < issued; ++taken) mbar_wait(bar + taken % SLOTS, (taken / SLOTS) & 1);
+  if (dead)  // copies in flight end before the CTA does
+    for (int i = 0; i < 4; ++i) mbar_wait(bar + i / 2, i & 1);
 }
 
-// Joins the segments of split sequences, one warp for a row's head, in
-// segment order.
-template <int HD, typename T, int PAIRS>
-__global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
-  constexpr int E = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const size_t unit = blockIdx.x * (size_t)(blockDim.x / 32) + threadIdx.x / 32;
-  griddep_wait();  // by every thread: the end of this kernel stands for the end of the one before it too
-  if (unit >= (size_t)p.c.n_rows * p.n_head) return;
-  const int row = (int)(unit / p.n_head), head = (int)(unit - (size_t)row * p.n_head);
-  const int s = kv4_seq_of(p.c, row);
-  if (s >= p.c.n_seq) return;
-  const int r0 = min(max(__ldg(p.c.row_start + s), 0), p.c.n_rows);
-  const int T_ = min(max(__ldg(p.c.row_start + s + 1), r0), p.c.n_rows) - r0;
-  const int L = min(max(__ldg(p.c.kv_len + s), 0), p.c.table_stride * KV_PAGE);
-  const Kv4Cut k = kv4_cut(L, T_, p.n_head / p.c.n_kv, p.c.n_kv, PAIRS, p.sms);
-  if (k.segs == 1 || row < r0) return;
-  const size_t slot = (size_t)r0 + (size_t)s * kv4_extra_slots(p.n_head, PAIRS, p.sms) + (size_t)(row - r0) * k.segs;
-  const float* src = p.part + (slot * p.n_head + head) * (HD + 4);
-  const size_t step = (size_t)p.n_head * (HD + 4);
-  float M = -INFINITY;
-  for (int j = lane; j < k.segs; j += 32) M = fmaxf(M, src[j * step]);
-  M = warp_max(M);
-  float ls = 0.0f, sum[E] = {};
-  for (int j = 0; j < k.segs; ++j) {
-    const float m = src[j * step], lj = src[j * step + 1];
-    if (m == -INFINITY && lj == 0.0f) continue;
-    const float by = exp2_approx(m - M);
-    ls = fmaf(lj, by, ls);
+// Joins the pieces of split runs, in the line's order: a CTA takes pairs of
+// runs in turn, its warps every 8th piece.
+constexpr int KV4_JOIN_WARPS = 8;
+template <int HD, typename T, int NT>
+__global__ void __launch_bounds__(KV4_JOIN_WARPS * 32) kv4_join_kernel(const Kv4AttnParams p) {
+  using A = Kv4Attn<HD, NT>;
+  constexpr int PAIRS = A::PAIRS, E = HD / 32, JW = KV4_JOIN_WARPS;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* red = reinterpret_cast<float*>(smem);              // [JW][HD + 1]
+  float* top = red + JW * (HD + 1);                         // [JW]
+  Kv4Line line;
+  line.page0 = reinterpret_cast<long long*>(smem + (JW * (HD + 1) + JW) * 4);
+  line.run0 = line.page0 + p.c.n_seq + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gqa = p.n_head / p.c.n_kv;
+  kv4_line<PAIRS>(p, line);  // of arrays that the attention does not write
+  griddep_wait();            // by every thread: the end of this kernel stands for the end of the attention too
+  const long long U = line.page0[p.c.n_seq], pairs = line.run0[p.c.n_seq] * PAIRS;
+  if (U == 0) return;
+  const int W = kv4_workers(U, p.ctas, A::NW);
+  for (long long x = blockIdx.x; x < pairs; x += gridDim.x) {
+    const long long run = x / PAIRS;
+    const int i = (int)(x - run * PAIRS), s = kv4_find(line.run0, p.c.n_seq, run);
+    const Kv4Seq q = kv4_seq<PAIRS>(p, s);
+    const int r = (int)(run - line.run0[s]), kv = r % p.c.n_kv, pr = r / p.c.n_kv * PAIRS + i;
+    const long long a = line.page0[s] + (long long)r * q.pages;
+    const int w0 = kv4_owner(a, U, W), w1 = kv4_owner(a + q.pages - 1, U, W);
+    if (w0 == w1 || pr >= q.T * gqa) continue;
+    auto piece = [&](int w) {
+      return p.part + (((size_t)w * 2 + (a <= kv4_first(w, U, W) ? 0 : 1)) * PAIRS + i) * A::PART;
+    };
+    float M = -INFINITY;
+    for (int w = w0 + threadIdx.x; w <= w1; w += JW * 32) M = fmaxf(M, *piece(w));
+    M = warp_max(M);
+    if (lane == 0) top[warp] = M;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < E; ++i) sum[i] = fmaf(src[j * step + 4 + lane * E + i], by, sum[i]);
+    for (int k = 0; k < JW; ++k) M = fmaxf(M, top[k]);
+    float l = 0.0f, sum[E] = {};
+#pragma unroll 4
+    for (int w = w0 + warp; w <= w1; w += JW) {
+      const float* src = piece(w);
+      const float2 ml = *reinterpret_cast<const float2*>(src);
+      // a piece that saw nothing counts for nothing
+      const float by = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : exp2_approx(ml.x - M);
+      l = fmaf(ml.y, by, l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] = fmaf(src[4 + e * 32 + lane], by, sum[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) red[warp * (HD + 1) + e * 32 + lane] = sum[e];
+    if (lane == 0) red[warp * (HD + 1) + HD] = l;
+    __syncthreads();
+    if (threadIdx.x < HD) {
+      float v = 0.0f, ls = 0.0f;
+#pragma unroll
+      for (int k = 0; k < JW; ++k) { v += red[k * (HD + 1) + threadIdx.x]; ls += red[k * (HD + 1) + HD]; }
+      static_cast<T*>(p.out)[((size_t)(q.r0 + pr / gqa) * p.n_head + kv * gqa + pr % gqa) * HD + threadIdx.x] =
+          (T)(ls == 0.0f ? 0.0f : __fdiv_rn(v, ls));
+    }
+    __syncthreads();
   }
-  T* out = static_cast<T*>(p.out) + unit * HD + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; ++i) out[i] = (T)(ls == 0.0f ? 0.0f : __fdiv_rn(sum[i], ls));
 }
 
 }  // namespace fox
