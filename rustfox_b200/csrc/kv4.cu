@@ -149,22 +149,23 @@ extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim) {
 }
 
 template <typename T, int HD, int NT>
-static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
+static cudaError_t launch_kv4_attend(Kv4AttnParams p, cudaStream_t s) {
   using A = Kv4Attn<HD, NT>;
+  p.whole = p.c.table_stride <= KV4_WHOLE_PAGES;
   const size_t smem = A::smem_bytes(p.c.n_seq);
   static size_t marks[kMaxDevices] = {}, join_marks[kMaxDevices] = {};
   cudaError_t e = opt_in_smem(kv4_attend_kernel<HD, T, NT>, smem, marks);
   if (e != cudaSuccess) return e;
   kv4_attend_kernel<HD, T, NT><<<p.ctas, A::NW * 32, smem, s>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if (p.c.table_stride <= KV4_MIN_PAGES) return e;  // no run can be split
+  if (p.whole) return e;
   // the join of split runs, its launch overlapped with the attention
   const int gqa = p.n_head / p.c.n_kv;
   const size_t most = ((size_t)p.c.n_rows * gqa / A::PAIRS + p.c.n_seq) * p.c.n_kv * A::PAIRS;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min<size_t>(most, (size_t)p.ctas * 4));
+  cfg.gridDim = dim3((unsigned)std::min<size_t>(most, (size_t)p.ctas * 8));
   cfg.blockDim = dim3(KV4_JOIN_WARPS * 32);
-  cfg.dynamicSmemBytes = (KV4_JOIN_WARPS * (HD + 1) + KV4_JOIN_WARPS) * 4 + (size_t)(p.c.n_seq + 1) * 16;
+  cfg.dynamicSmemBytes = kv4_join_smem<HD>(p.c.n_seq);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

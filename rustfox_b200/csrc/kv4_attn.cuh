@@ -22,12 +22,13 @@
 // - The scores of a 16-position step come out as (position, pair) per lane:
 //   the softmax needs no exchange but the maximum's, and 8x8 transposes turn
 //   its weights into the second product's operand.
-// - Odd positions of V are taken from their top level down, x = (m + 15 d) -
-//   d (15 - c), with the complement of the code (an xor that joins the mask)
-//   and a negated weight: the second product's sums then stay near the result
-//   instead of 7.5 d away from it. They round toward zero, so what would
-//   cancel in the end must not pass through them: at 32768 positions the error
-//   was 1e-4 of the result with all positions counted from below.
+// - Every second position of V is taken from its top level down, x = (m + 15
+//   d) - d (15 - c), with the complement of the code (an xor that joins the
+//   mask) and a negated weight, alternating within an operand and within what
+//   a lane sums: both sums then stay near the result instead of 7.5 d away
+//   from it. What cancels in the end must not pass through them: with all
+//   positions counted from below the error was 1e-4 of the result at 32768
+//   positions, now it is 1e-6.
 #pragma once
 
 #include <climits>
@@ -45,6 +46,7 @@ struct Kv4AttnParams {
   float* part;       // partial results of split runs, two a worker
   size_t q_stride;   // elements between rows
   int n_head, ctas;
+  int whole;         // runs are short: none is split
   float scale;
 };
 
@@ -56,7 +58,9 @@ struct Kv4AttnParams {
 // most two: the end of one run and the beginning of another) and are joined in
 // order by a second kernel. So the load is even whatever the lengths, and no
 // worker waits for another.
-constexpr int KV4_MIN_PAGES = 1;  // pages a worker takes at least
+// A second launch costs more than a few pages, so calls whose block tables
+// hold at most KV4_WHOLE_PAGES divide the line between runs.
+constexpr int KV4_MIN_PAGES = 1, KV4_WHOLE_PAGES = 4;  // pages a worker takes at least; of a run that is not split
 struct Kv4Line {
   long long* page0;  // [n_seq + 1] first page in line of each sequence
   long long* run0;   // [n_seq + 1] first run of each sequence
@@ -148,19 +152,20 @@ FOX_DEV uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h)
 
 // 8 codes of a word (nibble i in bits 4i) as four operand registers: codes
 // (0, 4), (1, 5), (2, 6), (3, 7), the even ones as c * 2^-22, the odd ones as
-// c * 2^-18. With ODD the upper half's codes are complemented.
-template <bool ODD>
+// c * 2^-18; FLIP: the halves whose codes are complemented.
+template <uint32_t FLIP>
 FOX_DEV void kv4_operands(uint32_t x, uint32_t (&a)[4]) {
-  constexpr uint32_t E = 0x003c003cu, O = 0x03c003c0u, FE = ODD ? E & 0xffff0000u : 0, FO = ODD ? O & 0xffff0000u : 0;
+  constexpr uint32_t E = 0x003c003cu, O = 0x03c003c0u;
   const uint32_t up = x << 2, down = x >> 6;
-  a[0] = (up & E) ^ FE;
-  a[1] = (up & O) ^ FO;
-  a[2] = (down & E) ^ FE;
-  a[3] = (down & O) ^ FO;
+  a[0] = (up & E) ^ (E & FLIP);
+  a[1] = (up & O) ^ (O & FLIP);
+  a[2] = (down & E) ^ (E & FLIP);
+  a[3] = (down & O) ^ (O & FLIP);
 }
 constexpr float KV4_EVEN = 4194304.0f;  // 2^22
 // A weight may exceed 1 by 2^SLACK before the sums are rescaled; times d it is
 // scaled to at most 2^15.
+constexpr int KV4_FLUSH = 4;
 constexpr float KV4_SLACK = 7.0f, KV4_WEIGHT = 256.0f;
 // x as hi + lo fp16: hi keeps the leading 11 bits.
 FOX_DEV uint32_t kv4_hi_lo(float x) {
@@ -185,11 +190,12 @@ struct Kv4Attn {
   static constexpr int SLAB = HD < 128 ? HD : 128, SLABS = HD / SLAB, SG = SLAB / 64, NB = SLAB / 32;
   static constexpr int G = HD / KV4_GROUP, BB = kv4_block_bytes(HD), PAGE_BYTES = 2 * BB;
   static constexpr int PAIRS = 4 * NT;       // (row, head) pairs of a tile
+  static constexpr int SUM_VECS = NT * SLABS * NB * 2;  // float4s of a lane's sums
   static constexpr int PART = HD + 4;        // floats of one pair's partial result: M, l, -, -, sums
   // warps of a CTA, each with room for a page's K and V: what the registers hold
   static constexpr int NW = HD < 256 ? 12 : 8;
   static constexpr size_t smem_bytes(int n_seq) {
-    return (size_t)NW * PAGE_BYTES + NW * 2 * 8 + (size_t)(n_seq + 1) * 16;
+    return (size_t)NW * (PAGE_BYTES + SUM_VECS * 512) + NW * 2 * 8 + (size_t)(n_seq + 1) * 16;
   }
 
   // A warp's share of a tile: q's operand registers, and the running maximum,
@@ -199,6 +205,11 @@ struct Kv4Attn {
   uint32_t qb[NT][SLABS][SG][2][2][2];
   float f[NT], qs[NT][G];  // score = f * sum_g (d_g * product) + sum_g m_g * qs_g, in powers of 2
   float o[NT][SLABS][NB][2][4], mx[NT], l[NT], mo[NT][G], big;
+  // The matrix instructions round their sums toward zero, 0.7 * 2^-24 of them
+  // each time, so after KV4_FLUSH pages they move to shared memory (this
+  // lane's float4s, 32 apart), added to the nearest. `flushed`: there are any.
+  float4* sums;
+  bool flushed;
   float sco[NT][4][2];            // the page's scores
   int lim[NT], lim_min, lim_max;  // the last position a pair sees (negative: none; no pair: all), and over the tile
 
@@ -278,6 +289,32 @@ struct Kv4Attn {
       for (int j = 0; j < G; ++j) mo[n][j] = 0.0f;
     }
     big = 0x1p-24f;  // a power of two above every d met
+    flushed = false;
+  }
+
+  FOX_DEV float4 sum_of(int n, int sl, int b, int h) const {
+    const float(&c)[4] = o[n][sl][b][h];
+    float4 v = make_float4(c[0], c[1], c[2], c[3]);
+    if (flushed) {
+      const float4 w = sums[32 * (((n * SLABS + sl) * NB + b) * 2 + h)];
+      v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    }
+    return v;
+  }
+  FOX_DEV void flush() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int sl = 0; sl < SLABS; ++sl)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            sums[32 * (((n * SLABS + sl) * NB + b) * 2 + h)] = sum_of(n, sl, b, h);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[n][sl][b][h][c] = 0.0f;
+          }
+    flushed = true;
   }
 
   // The scores of a page's K block.
@@ -306,8 +343,8 @@ struct Kv4Attn {
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             uint32_t x[4], y[4];
-            kv4_operands<false>(wa[2 * j + w], x);
-            kv4_operands<false>(wb[2 * j + w], y);
+            kv4_operands<0>(wa[2 * j + w], x);
+            kv4_operands<0>(wb[2 * j + w], y);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint32_t(&b)[2][2] = qb[n][sl][j][w];
@@ -393,27 +430,36 @@ struct Kv4Attn {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int c = 0; c < 4; ++c) o[n][sl][b][h][c] *= all;
+        if (flushed)
+#pragma unroll
+          for (int i = 0; i < SUM_VECS / NT; ++i) {
+            float4& v = sums[32 * (n * (SUM_VECS / NT) + i)];
+            v = make_float4(v.x * all, v.y * all, v.z * all, v.w * all);
+          }
       }
     }
 
     // the weights, times d, as the second product's operand
     const float norm = ((g & 1) ? -KV4_WEIGHT : KV4_WEIGHT) / big, from_top = (g & 1) ? 15.0f : 0.0f;
+    // which positions count from the top: odd ones of a step's first half and
+    // even ones of its second, the other way round in the next step
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       uint32_t pb[NT][G][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        const bool swap = (s + h) & 1;
         float w[NT], wn[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           w[n] = exp2_approx(sco[n][s][h] - (EDGE && mx[n] == -INFINITY ? 0.0f : mx[n]));
-          wn[n] = w[n] * norm;
+          wn[n] = w[n] * (swap ? -norm : norm);
           l[n] += w[n];
         }
 #pragma unroll
         for (int j = 0; j < G; ++j) {
           const float2 d = __half22float2(dv[s][h][j]);
-          const float m = fmaf(from_top, d.x, d.y);
+          const float m = fmaf(swap ? 15.0f - from_top : from_top, d.x, d.y);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const bool hidden = EDGE && sco[n][s][h] == -INFINITY;  // whatever it is
@@ -437,8 +483,13 @@ struct Kv4Attn {
         for (int b = 0; b < NB; ++b) {
           const int j = sl * SG + b / 2;
           uint32_t x[4], y[4];
-          kv4_operands<true>(u[b], x);
-          kv4_operands<true>(v[b], y);
+          if (s & 1) {
+            kv4_operands<0x0000ffffu>(u[b], x);
+            kv4_operands<0xffff0000u>(v[b], y);
+          } else {
+            kv4_operands<0xffff0000u>(u[b], x);
+            kv4_operands<0x0000ffffu>(v[b], y);
+          }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma16816(o[n][sl][b][0], x[0], x[1], y[0], y[1], pb[n][j][0], pb[n][j][1]);
@@ -472,9 +523,9 @@ struct Kv4Attn {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const float m = mo[n][sl * SG + b / 2];
-          const float(&c)[2][4] = o[n][sl][b];
-          float4 v = make_float4(fmaf(c[0][0] + c[0][1], unit, m), fmaf(c[0][2] + c[0][3], unit * 0.0625f, m),
-                                 fmaf(c[1][0] + c[1][1], unit, m), fmaf(c[1][2] + c[1][3], unit * 0.0625f, m));
+          const float4 x = sum_of(n, sl, b, 0), y = sum_of(n, sl, b, 1);
+          const float4 v = make_float4(fmaf(x.x + x.y, unit, m), fmaf(x.z + x.w, unit * 0.0625f, m),
+                                       fmaf(y.x + y.y, unit, m), fmaf(y.z + y.w, unit * 0.0625f, m));
           const int d = sl * SLAB + b * 32 + g * 4;
           if (part) *reinterpret_cast<float4*>(dst + 4 + d) = v;
           else kv4_store4(out + d, kv4_quotient(v, l[n]));
@@ -491,9 +542,10 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint8_t* ring = smem + (size_t)warp * A::PAGE_BYTES;
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + (size_t)NW * A::PAGE_BYTES) + warp * 2;
+  uint8_t* behind = smem + (size_t)NW * (A::PAGE_BYTES + A::SUM_VECS * 512);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(behind) + warp * 2;
   Kv4Line line;
-  line.page0 = reinterpret_cast<long long*>(smem + (size_t)NW * A::PAGE_BYTES + NW * 2 * 8);
+  line.page0 = reinterpret_cast<long long*>(behind + NW * 2 * 8);
   line.run0 = line.page0 + p.c.n_seq + 1;
   const int gqa = p.n_head / p.c.n_kv;
 
@@ -509,9 +561,18 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
   const long long U = line.page0[p.c.n_seq];
   if (U == 0) return;
   // neighbours in line sit on different SMs
-  const int W = kv4_workers(U, gridDim.x, NW), worker = warp * gridDim.x + blockIdx.x;
+  const long long runs = line.run0[p.c.n_seq];
+  const int W = p.whole ? (int)min((long long)gridDim.x * NW, runs) : kv4_workers(U, gridDim.x, NW);
+  const int worker = warp * gridDim.x + blockIdx.x;
   if (worker >= W) return;
-  const long long u0 = kv4_first(worker, U, W), u1 = kv4_first(worker + 1, U, W);
+  auto edge = [&](long long w) {
+    if (!p.whole) return kv4_first(w, U, W);
+    const long long run = kv4_first(w, runs, W);
+    if (run == runs) return U;
+    const int s = kv4_find(line.run0, p.c.n_seq, run);
+    return line.page0[s] + (run - line.run0[s]) * kv4_seq<PAIRS>(p, s).pages;
+  };
+  const long long u0 = edge(worker), u1 = edge(worker + 1);
 
   auto locate = [&](long long u) {
     Kv4Unit x;
@@ -546,6 +607,8 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
   };
 
   A w;
+  w.sums = reinterpret_cast<float4*>(smem + (size_t)NW * A::PAGE_BYTES) + warp * A::SUM_VECS * 32 + lane;
+  int since = 0;       // pages whose sums are in registers
   Kv4Unit cur = locate(u0);
   const uint8_t* block = find(cur);
   ask(block, 0);
@@ -571,6 +634,7 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
       __syncwarp();
       if (!dead) ask(after, 1);
       phase ^= 1;
+      if (++since == KV4_FLUSH) { w.flush(); since = 0; }
     } else {
       ask(after, 0);
       ask(after, 1);
@@ -581,6 +645,7 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
       float* part = p.part + ((size_t)worker * 2 + (run_first <= u0 ? 0 : 1)) * (PAIRS * A::PART);
       w.template end<T>(p, cur, gqa, whole ? nullptr : part);
       if (!last) w.template begin<T>(p, nxt, gqa);
+      since = 0;
     }
     cur = nxt;
     block = dead ? nullptr : after;
@@ -589,18 +654,22 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
     for (int i = 0; i < 4; ++i) mbar_wait(bar + i / 2, i & 1);
 }
 
-// Joins the pieces of split runs, in the line's order: a CTA takes pairs of
-// runs in turn, its warps every 8th piece.
+// Joins the pieces of split runs, in the line's order. A pair of a run takes
+// 1, 2, 4 or 8 of the CTA's warps, by how many pieces a run has on average;
+// each takes every such-th piece.
 constexpr int KV4_JOIN_WARPS = 8;
+template <int HD>
+__host__ __device__ constexpr int kv4_join_smem(int n_seq) {
+  return KV4_JOIN_WARPS * (HD + 2) * 4 + (n_seq + 1) * 16;
+}
 template <int HD, typename T, int NT>
 __global__ void __launch_bounds__(KV4_JOIN_WARPS * 32) kv4_join_kernel(const Kv4AttnParams p) {
   using A = Kv4Attn<HD, NT>;
   constexpr int PAIRS = A::PAIRS, E = HD / 32, JW = KV4_JOIN_WARPS;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem);              // [JW][HD + 1]
-  float* top = red + JW * (HD + 1);                         // [JW]
+  float* red = reinterpret_cast<float*>(smem);  // [JW][HD + 2]
   Kv4Line line;
-  line.page0 = reinterpret_cast<long long*>(smem + (JW * (HD + 1) + JW) * 4);
+  line.page0 = reinterpret_cast<long long*>(smem + JW * (HD + 2) * 4);
   line.run0 = line.page0 + p.c.n_seq + 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gqa = p.n_head / p.c.n_kv;
   kv4_line<PAIRS>(p, line);  // of arrays that the attention does not write
@@ -608,47 +677,55 @@ __global__ void __launch_bounds__(KV4_JOIN_WARPS * 32) kv4_join_kernel(const Kv4
   const long long U = line.page0[p.c.n_seq], pairs = line.run0[p.c.n_seq] * PAIRS;
   if (U == 0) return;
   const int W = kv4_workers(U, p.ctas, A::NW);
-  for (long long x = blockIdx.x; x < pairs; x += gridDim.x) {
-    const long long run = x / PAIRS;
-    const int i = (int)(x - run * PAIRS), s = kv4_find(line.run0, p.c.n_seq, run);
-    const Kv4Seq q = kv4_seq<PAIRS>(p, s);
-    const int r = (int)(run - line.run0[s]), kv = r % p.c.n_kv, pr = r / p.c.n_kv * PAIRS + i;
-    const long long a = line.page0[s] + (long long)r * q.pages;
-    const int w0 = kv4_owner(a, U, W), w1 = kv4_owner(a + q.pages - 1, U, W);
-    if (w0 == w1 || pr >= q.T * gqa) continue;
-    auto piece = [&](int w) {
-      return p.part + (((size_t)w * 2 + (a <= kv4_first(w, U, W) ? 0 : 1)) * PAIRS + i) * A::PART;
-    };
-    float M = -INFINITY;
-    for (int w = w0 + threadIdx.x; w <= w1; w += JW * 32) M = fmaxf(M, *piece(w));
-    M = warp_max(M);
-    if (lane == 0) top[warp] = M;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < JW; ++k) M = fmaxf(M, top[k]);
+  int team = 1;  // warps of a pair
+  while (team < JW && (long long)team * 8 * line.run0[p.c.n_seq] < W) team *= 2;
+  const int teams = JW / team, in_team = warp % team;
+  for (long long x0 = (long long)blockIdx.x * teams; x0 < pairs; x0 += (long long)gridDim.x * teams) {
+    const long long x = x0 + warp / team, run = x / PAIRS;
     float l = 0.0f, sum[E] = {};
+    T* out = nullptr;
+    if (x < pairs) {
+      const int i = (int)(x - run * PAIRS), s = kv4_find(line.run0, p.c.n_seq, run);
+      const Kv4Seq q = kv4_seq<PAIRS>(p, s);
+      const int r = (int)(run - line.run0[s]), kv = r % p.c.n_kv, pr = r / p.c.n_kv * PAIRS + i;
+      const long long a = line.page0[s] + (long long)r * q.pages;
+      const int w0 = kv4_owner(a, U, W), w1 = kv4_owner(a + q.pages - 1, U, W);
+      if (w0 != w1 && pr < q.T * gqa) {
+        out = static_cast<T*>(p.out) + ((size_t)(q.r0 + pr / gqa) * p.n_head + kv * gqa + pr % gqa) * HD;
+        // a run's first piece may be the second of its worker; the others are their workers' first
+        const float* head = p.part + (((size_t)w0 * 2 + (a <= kv4_first(w0, U, W) ? 0 : 1)) * PAIRS + i) * A::PART;
+        auto piece = [&](int w) { return w == w0 ? head : p.part + ((size_t)w * 2 * PAIRS + i) * A::PART; };
+        float M = -INFINITY;
+        for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, *piece(w));
+        M = warp_max(M);
 #pragma unroll 4
-    for (int w = w0 + warp; w <= w1; w += JW) {
-      const float* src = piece(w);
-      const float2 ml = *reinterpret_cast<const float2*>(src);
-      // a piece that saw nothing counts for nothing
-      const float by = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : exp2_approx(ml.x - M);
-      l = fmaf(ml.y, by, l);
+        for (int w = w0 + in_team; w <= w1; w += team) {
+          const float* src = piece(w);
+          const float2 ml = *reinterpret_cast<const float2*>(src);
+          // a piece that saw nothing counts for nothing
+          const float by = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : exp2_approx(ml.x - M);
+          l = fmaf(ml.y, by, l);
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum[e] = fmaf(src[4 + e * 32 + lane], by, sum[e]);
+          for (int e = 0; e < E; ++e) sum[e] = fmaf(src[4 + e * 32 + lane], by, sum[e]);
+        }
+      }
     }
+    if (team > 1) {
+      __syncthreads();  // red is free
 #pragma unroll
-    for (int e = 0; e < E; ++e) red[warp * (HD + 1) + e * 32 + lane] = sum[e];
-    if (lane == 0) red[warp * (HD + 1) + HD] = l;
-    __syncthreads();
-    if (threadIdx.x < HD) {
-      float v = 0.0f, ls = 0.0f;
+      for (int e = 0; e < E; ++e) red[warp * (HD + 2) + e * 32 + lane] = sum[e];
+      if (lane == 0) red[warp * (HD + 2) + HD] = l;
+      __syncthreads();
+      if (in_team) continue;
+      for (int k = 1; k < team; ++k) {
+        l += red[(warp + k) * (HD + 2) + HD];
 #pragma unroll
-      for (int k = 0; k < JW; ++k) { v += red[k * (HD + 1) + threadIdx.x]; ls += red[k * (HD + 1) + HD]; }
-      static_cast<T*>(p.out)[((size_t)(q.r0 + pr / gqa) * p.n_head + kv * gqa + pr % gqa) * HD + threadIdx.x] =
-          (T)(ls == 0.0f ? 0.0f : __fdiv_rn(v, ls));
+        for (int e = 0; e < E; ++e) sum[e] += red[(warp + k) * (HD + 2) + e * 32 + lane];
+      }
     }
-    __syncthreads();
+    if (out)
+#pragma unroll
+      for (int e = 0; e < E; ++e) out[e * 32 + lane] = (T)(l == 0.0f ? 0.0f : __fdiv_rn(sum[e], l));
   }
 }
 
