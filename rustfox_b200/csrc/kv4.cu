@@ -131,19 +131,23 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
   return FOXCUDA_OK;
 }
 
-// Two partial results of a tile for every worker.
+// A tile's pieces: two of every CTA, and one of every warp.
 template <int HD, int NT>
-static size_t kv4_part_bytes(int ctas) {
+static size_t kv4_piece_floats(int ctas, int each) {
   using A = Kv4Attn<HD, NT>;
-  return (size_t)ctas * A::NW * 2 * A::PAIRS * A::PART * 4;
+  return (size_t)ctas * each * A::PAIRS * A::PART;
+}
+template <int HD, int NT>
+static size_t kv4_work_bytes(int ctas) {
+  return kv4_piece_floats<HD, NT>(ctas, 2 + Kv4Attn<HD, NT>::NW) * 4;
 }
 
 extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim) {
   const int ctas = current_sms();
   switch (head_dim) {
-    case 64: return kv4_part_bytes<64, 1>(ctas);
-    case 128: return kv4_part_bytes<128, 1>(ctas);
-    case 256: return kv4_part_bytes<256, 1>(ctas);
+    case 64: return kv4_work_bytes<64, 1>(ctas);
+    case 128: return kv4_work_bytes<128, 1>(ctas);
+    case 256: return kv4_work_bytes<256, 1>(ctas);
     default: return 0;
   }
 }
@@ -151,14 +155,14 @@ extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim) {
 template <typename T, int HD, int NT>
 static cudaError_t launch_kv4_attend(Kv4AttnParams p, cudaStream_t s) {
   using A = Kv4Attn<HD, NT>;
-  p.whole = p.c.table_stride <= KV4_WHOLE_PAGES;
+  p.heads = p.part + kv4_piece_floats<HD, NT>(p.ctas, 2);
   const size_t smem = A::smem_bytes(p.c.n_seq);
   static size_t marks[kMaxDevices] = {}, join_marks[kMaxDevices] = {};
   cudaError_t e = opt_in_smem(kv4_attend_kernel<HD, T, NT>, smem, marks);
   if (e != cudaSuccess) return e;
   kv4_attend_kernel<HD, T, NT><<<p.ctas, A::NW * 32, smem, s>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if (p.whole) return e;
+  if (p.c.table_stride <= KV4_WHOLE) return e;  // no run is split between CTAs
   // the join of split runs, its launch overlapped with the attention
   const int gqa = p.n_head / p.c.n_kv;
   const size_t most = ((size_t)p.c.n_rows * gqa / A::PAIRS + p.c.n_seq) * p.c.n_kv * A::PAIRS;
@@ -192,6 +196,11 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) ||
       !stride_ok(q_stride, (size_t)n_head * c->head_dim, type))
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: rows and workspace must be 16-byte aligned, rows at least a row apart");
+  // tiles of at least 4 (row, head) pairs, each with every page of its sequence
+  const double units = ((double)c->n_rows * gqa / 4 + c->n_seq) * c->n_head_kv * ((double)c->table_stride + KV4_HEAD);
+  if (units >= 2147483648.0)
+    return fail(FOXCUDA_ERR_ARG, "kv4_attention: %u rows over %u pages a sequence are too many for one call",
+                c->n_rows, c->table_stride);
   const size_t need = foxcuda_kv4_attention_workspace(c->head_dim);
   if (workspace_bytes < need)
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: the workspace holds %zu bytes, %zu are needed", workspace_bytes, need);

@@ -43,29 +43,28 @@ struct Kv4AttnParams {
   Kv4Rows c;
   const void* q;
   void* out;
-  float* part;       // partial results of split runs, two a worker
-  size_t q_stride;   // elements between rows
+  float *part, *heads;  // workspace: pieces of runs split over CTAs, and over a CTA's warps
+  size_t q_stride;      // elements between rows
   int n_head, ctas;
-  int whole;         // runs are short: none is split
   float scale;
 };
 
 // How the work is divided. A tile is PAIRS (row, head) pairs of one KV head of
-// a sequence, a run all the pages of its sequence, and a warp is a worker:
-// the runs stand in a line (sequence, tile, KV head), and every worker takes
-// an equal stretch of the line's pages. A worker that holds a whole run writes
-// its result; the pieces of a split one go to the workspace (a worker holds at
-// most two: the end of one run and the beginning of another) and are joined in
-// order by a second kernel. So the load is even whatever the lengths, and no
-// worker waits for another.
-// A second launch costs more than a few pages, so calls whose block tables
-// hold at most KV4_WHOLE_PAGES divide the line between runs.
-constexpr int KV4_MIN_PAGES = 1, KV4_WHOLE_PAGES = 4;  // pages a worker takes at least; of a run that is not split
-struct Kv4Line {
-  long long* page0;  // [n_seq + 1] first page in line of each sequence
-  long long* run0;   // [n_seq + 1] first run of each sequence
-};
-struct Kv4Seq { int r0, T, L, tiles, pages; };
+// a sequence, a run all the pages of its sequence. The runs stand in a line
+// (sequence, tile, KV head); every CTA takes an equal stretch of it, and every
+// warp an equal stretch of its CTA's, so the load is even whatever the lengths
+// and no warp waits for another before its end. A warp's stretch holds whole
+// runs, whose results it writes, and at most two pieces: the end of one run and
+// the beginning of another. The CTA joins its warps' pieces in shared memory,
+// and a second kernel joins, in order, the CTAs' pieces of runs that are split
+// between CTAs. That launch costs more than a few pages' work: a line without
+// a run of more than KV4_WHOLE pages is divided between runs, and no second
+// kernel follows where the block tables hold no more.
+constexpr int KV4_WHOLE = 16;
+// A run begins with KV4_HEAD units without a page: what its queries' loading
+// and its results' writing take of a worker's time.
+constexpr int KV4_HEAD = 2;
+struct Kv4Seq { int r0, T, L, tiles, units; };
 
 template <int PAIRS>
 FOX_DEV Kv4Seq kv4_seq(const Kv4AttnParams& p, int s) {
@@ -74,56 +73,79 @@ FOX_DEV Kv4Seq kv4_seq(const Kv4AttnParams& p, int s) {
   q.T = min(max(__ldg(p.c.row_start + s + 1), q.r0), p.c.n_rows) - q.r0;
   q.L = kv4_len(p.c, s);
   q.tiles = (q.T * (p.n_head / p.c.n_kv) + PAIRS - 1) / PAIRS;
-  q.pages = max(1, (q.L + KV_PAGE - 1) / KV_PAGE);  // one even where nothing is cached: its rows get zeros
+  q.units = KV4_HEAD + (q.L + KV_PAGE - 1) / KV_PAGE;
   return q;
 }
 
-// Prefix sums of the sequences' runs and pages, by the CTA's first warp.
-template <int PAIRS>
-FOX_DEV void kv4_line(const Kv4AttnParams& p, const Kv4Line& line) {
-  const int lane = threadIdx.x & 31;
-  if (threadIdx.x < 32) {
-    long long runs = 0, pages = 0;
-    for (int s0 = 0; s0 < p.c.n_seq; s0 += 32) {
-      const int s = s0 + lane;
-      long long r = 0, n = 0;
-      if (s < p.c.n_seq) {
-        const Kv4Seq q = kv4_seq<PAIRS>(p, s);
-        r = (long long)q.tiles * p.c.n_kv;
-        n = r * q.pages;
-      }
-      long long rs = r, ns = n;
+// n things in `parts` nearly equal stretches. The host keeps every count of
+// units below 2^31.
+struct Kv4Split {
+  int base, rem;
+  FOX_DEV Kv4Split(int n, int parts) : base(n / parts), rem(n - n / parts * parts) {}
+  FOX_DEV int first(int i) const { return i * base + min(i, rem); }
+  FOX_DEV int owner(int u) const {
+    const int wide = rem * (base + 1);
+    return u < wide ? u / (base + 1) : rem + (u - wide) / base;
+  }
+};
+
+// The line: the first unit and run of each sequence (n_seq + 1 each, then the
+// longest sequence's units), in shared memory.
+struct Kv4Line {
+  int *unit0, *run0;
+  int U, runs, n_seq;
+  bool whole;  // no run is split between CTAs
+  static __host__ __device__ int bytes(int n_seq) { return (2 * n_seq + 3) * 4; }
+
+  // By the CTA's first warp; every thread calls.
+  template <int PAIRS>
+  FOX_DEV void build(const Kv4AttnParams& p, void* mem) {
+    n_seq = p.c.n_seq;
+    unit0 = static_cast<int*>(mem);
+    run0 = unit0 + n_seq + 1;
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {
+      int r0 = 0, u0 = 0, longest = 0;
+      for (int s0 = 0; s0 < n_seq; s0 += 32) {
+        const int s = s0 + lane;
+        int r = 0, n = 0;
+        if (s < n_seq) {
+          const Kv4Seq q = kv4_seq<PAIRS>(p, s);
+          r = q.tiles * p.c.n_kv;
+          n = r * q.units;
+          if (r) longest = max(longest, q.units);
+        }
+        int rs = r, ns = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long ru = __shfl_up_sync(0xffffffffu, rs, o), nu = __shfl_up_sync(0xffffffffu, ns, o);
-        if (lane >= o) { rs += ru; ns += nu; }
+        for (int o = 1; o < 32; o <<= 1) {
+          const int ru = __shfl_up_sync(0xffffffffu, rs, o), nu = __shfl_up_sync(0xffffffffu, ns, o);
+          if (lane >= o) { rs += ru; ns += nu; }
+        }
+        if (s < n_seq) { run0[s] = r0 + rs - r; unit0[s] = u0 + ns - n; }
+        r0 += __shfl_sync(0xffffffffu, rs, 31);
+        u0 += __shfl_sync(0xffffffffu, ns, 31);
       }
-      if (s < p.c.n_seq) { line.run0[s] = runs + rs - r; line.page0[s] = pages + ns - n; }
-      runs += __shfl_sync(0xffffffffu, rs, 31);
-      pages += __shfl_sync(0xffffffffu, ns, 31);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+      if (lane == 0) { run0[n_seq] = r0; unit0[n_seq] = u0; run0[n_seq + 1] = longest; }
     }
-    if (lane == 0) { line.run0[p.c.n_seq] = runs; line.page0[p.c.n_seq] = pages; }
+    __syncthreads();
+    runs = run0[n_seq];
+    U = unit0[n_seq];
+    whole = run0[n_seq + 1] <= KV4_HEAD + KV4_WHOLE;
   }
-  __syncthreads();
-}
-
-// The last sequence that begins at or before x (sequences without runs take
-// no room, so it is the one that holds x).
-FOX_DEV int kv4_find(const long long* start, int n_seq, long long x) {
-  int lo = 0, hi = n_seq - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (start[mid] <= x) lo = mid; else hi = mid - 1;
+  // The last sequence that begins at or before x (sequences without runs take
+  // no room, so it is the one that holds x).
+  FOX_DEV int find(const int* start, int x) const {
+    int lo = 0, hi = n_seq - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (start[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
   }
-  return lo;
-}
-
-// Worker w of W takes pages w * U / W .. (w + 1) * U / W - 1 of the line's U.
-FOX_DEV int kv4_workers(long long U, int ctas, int nw) {
-  return (int)min((long long)ctas * nw, (U + KV4_MIN_PAGES - 1) / KV4_MIN_PAGES);
-}
-FOX_DEV long long kv4_first(long long w, long long U, int W) { return w * U / W; }
-FOX_DEV int kv4_owner(long long u, long long U, int W) { return (int)(((u + 1) * W - 1) / U); }
+  FOX_DEV int ctas(int most) const { return min(most, whole ? runs : U / 2); }
+};
 
 FOX_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -150,22 +172,36 @@ FOX_DEV float exp2_approx(float x) {
 }
 FOX_DEV uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
+// (x & mask) ^ flip in one instruction, flip from a register.
+template <uint32_t MASK>
+FOX_DEV uint32_t kv4_pick(uint32_t x, uint32_t flip) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(x), "n"(MASK), "r"(flip));
+  return r;
+}
+constexpr uint32_t KV4_E = 0x003c003cu, KV4_O = 0x03c003c0u;
 // 8 codes of a word (nibble i in bits 4i) as four operand registers: codes
 // (0, 4), (1, 5), (2, 6), (3, 7), the even ones as c * 2^-22, the odd ones as
-// c * 2^-18; FLIP: the halves whose codes are complemented.
-template <uint32_t FLIP>
+// c * 2^-18; flip_e and flip_o: the masks' bits in the halves whose codes are
+// complemented.
 FOX_DEV void kv4_operands(uint32_t x, uint32_t (&a)[4]) {
-  constexpr uint32_t E = 0x003c003cu, O = 0x03c003c0u;
   const uint32_t up = x << 2, down = x >> 6;
-  a[0] = (up & E) ^ (E & FLIP);
-  a[1] = (up & O) ^ (O & FLIP);
-  a[2] = (down & E) ^ (E & FLIP);
-  a[3] = (down & O) ^ (O & FLIP);
+  a[0] = up & KV4_E;
+  a[1] = up & KV4_O;
+  a[2] = down & KV4_E;
+  a[3] = down & KV4_O;
+}
+FOX_DEV void kv4_operands(uint32_t x, uint32_t flip_e, uint32_t flip_o, uint32_t (&a)[4]) {
+  const uint32_t up = x << 2, down = x >> 6;
+  a[0] = kv4_pick<KV4_E>(up, flip_e);
+  a[1] = kv4_pick<KV4_O>(up, flip_o);
+  a[2] = kv4_pick<KV4_E>(down, flip_e);
+  a[3] = kv4_pick<KV4_O>(down, flip_o);
 }
 constexpr float KV4_EVEN = 4194304.0f;  // 2^22
+constexpr int KV4_FLUSH = 4;  // pages whose sums stay in the matrix instructions' registers
 // A weight may exceed 1 by 2^SLACK before the sums are rescaled; times d it is
 // scaled to at most 2^15.
-constexpr int KV4_FLUSH = 4;
 constexpr float KV4_SLACK = 7.0f, KV4_WEIGHT = 256.0f;
 // x as hi + lo fp16: hi keeps the leading 11 bits.
 FOX_DEV uint32_t kv4_hi_lo(float x) {
@@ -173,16 +209,44 @@ FOX_DEV uint32_t kv4_hi_lo(float x) {
   return half2_bits(__floats2half2_rn(hi, x - hi));
 }
 
-// A page in line: page `page` of a run.
+// A unit in line: page `page` of a run, or its head (negative).
 struct Kv4Unit {
   Kv4Seq q;
-  int seq, tile, kv, page;
+  int seq, run, tile, kv, page;
 };
 
 FOX_DEV float4 kv4_quotient(float4 v, float l) {
   if (l == 0.0f) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // nothing to see
   return make_float4(__fdiv_rn(v.x, l), __fdiv_rn(v.y, l), __fdiv_rn(v.z, l), __fdiv_rn(v.w, l));
 }
+
+// Pieces of a pair's results joined one after the other: M, l and, of the
+// sums, dimensions lane, lane + 32, ...
+template <int HD>
+struct Kv4Sum {
+  float M = -INFINITY, l = 0.0f, v[HD / 32] = {};
+  FOX_DEV void add(float m, float lm, const float (&x)[HD / 32]) {
+    if (m == -INFINITY && lm == 0.0f) return;  // a piece that saw nothing
+    const float to = fmaxf(M, m), old = M == -INFINITY ? 0.0f : exp2_approx(M - to), by = exp2_approx(m - to);
+    M = to;
+    l = fmaf(l, old, lm * by);
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) v[e] = fmaf(v[e], old, x[e] * by);
+  }
+  FOX_DEV void add(const float* piece) {
+    const float2 ml = *reinterpret_cast<const float2*>(piece);
+    float x[HD / 32];
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) x[e] = piece[4 + e * 32 + (threadIdx.x & 31)];
+    add(ml.x, ml.y, x);
+  }
+  template <typename T>
+  FOX_DEV void store(T* out) const {
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e)
+      out[e * 32 + (threadIdx.x & 31)] = (T)(l == 0.0f ? 0.0f : __fdiv_rn(v[e], l));
+  }
+};
 
 // HD: head dimension; NT: column tiles (of 4 pairs) of a warp.
 template <int HD, int NT>
@@ -195,7 +259,7 @@ struct Kv4Attn {
   // warps of a CTA, each with room for a page's K and V: what the registers hold
   static constexpr int NW = HD < 256 ? 12 : 8;
   static constexpr size_t smem_bytes(int n_seq) {
-    return (size_t)NW * (PAGE_BYTES + SUM_VECS * 512) + NW * 2 * 8 + (size_t)(n_seq + 1) * 16;
+    return (size_t)NW * (PAGE_BYTES + SUM_VECS * 512) + NW * 2 * 8 + NW * 2 * 4 + Kv4Line::bytes(n_seq);
   }
 
   // A warp's share of a tile: q's operand registers, and the running maximum,
@@ -343,8 +407,8 @@ struct Kv4Attn {
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             uint32_t x[4], y[4];
-            kv4_operands<0>(wa[2 * j + w], x);
-            kv4_operands<0>(wb[2 * j + w], y);
+            kv4_operands(wa[2 * j + w], x);
+            kv4_operands(wb[2 * j + w], y);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint32_t(&b)[2][2] = qb[n][sl][j][w];
@@ -443,6 +507,9 @@ struct Kv4Attn {
     const float norm = ((g & 1) ? -KV4_WEIGHT : KV4_WEIGHT) / big, from_top = (g & 1) ? 15.0f : 0.0f;
     // which positions count from the top: odd ones of a step's first half and
     // even ones of its second, the other way round in the next step
+    uint32_t flip[2][2] = {{KV4_E & 0xffff0000u, KV4_O & 0xffff0000u}, {KV4_E & 0xffffu, KV4_O & 0xffffu}};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+r"(flip[i / 2][i % 2]));  // held in registers
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       uint32_t pb[NT][G][2];
@@ -483,13 +550,8 @@ struct Kv4Attn {
         for (int b = 0; b < NB; ++b) {
           const int j = sl * SG + b / 2;
           uint32_t x[4], y[4];
-          if (s & 1) {
-            kv4_operands<0x0000ffffu>(u[b], x);
-            kv4_operands<0xffff0000u>(v[b], y);
-          } else {
-            kv4_operands<0xffff0000u>(u[b], x);
-            kv4_operands<0x0000ffffu>(v[b], y);
-          }
+          kv4_operands(u[b], flip[s & 1][0], flip[s & 1][1], x);
+          kv4_operands(v[b], flip[1 - (s & 1)][0], flip[1 - (s & 1)][1], y);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma16816(o[n][sl][b][0], x[0], x[1], y[0], y[1], pb[n][j][0], pb[n][j][1]);
@@ -538,58 +600,55 @@ struct Kv4Attn {
 template <int HD, typename T, int NT>
 __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel(const Kv4AttnParams p) {
   using A = Kv4Attn<HD, NT>;
-  constexpr int PAIRS = A::PAIRS, NW = A::NW;
+  constexpr int PAIRS = A::PAIRS, NW = A::NW, E = HD / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint8_t* ring = smem + (size_t)warp * A::PAGE_BYTES;
   uint8_t* behind = smem + (size_t)NW * (A::PAGE_BYTES + A::SUM_VECS * 512);
   uint64_t* bar = reinterpret_cast<uint64_t*>(behind) + warp * 2;
+  int* piece_run = reinterpret_cast<int*>(behind + NW * 2 * 8);  // [2 NW], in line: the runs of the warps' pieces, or -1
   Kv4Line line;
-  line.page0 = reinterpret_cast<long long*>(behind + NW * 2 * 8);
-  line.run0 = line.page0 + p.c.n_seq + 1;
   const int gqa = p.n_head / p.c.n_kv;
 
   if (lane == 0) {
     mbar_init(bar, 1);
     mbar_init(bar + 1, 1);
     mbar_fence_init();
+    piece_run[2 * warp] = piece_run[2 * warp + 1] = -1;
   }
   __syncwarp();
   griddep_wait();
   griddep_launch_dependents();
-  kv4_line<PAIRS>(p, line);
-  const long long U = line.page0[p.c.n_seq];
-  if (U == 0) return;
-  // neighbours in line sit on different SMs
-  const long long runs = line.run0[p.c.n_seq];
-  const int W = p.whole ? (int)min((long long)gridDim.x * NW, runs) : kv4_workers(U, gridDim.x, NW);
-  const int worker = warp * gridDim.x + blockIdx.x;
-  if (worker >= W) return;
-  auto edge = [&](long long w) {
-    if (!p.whole) return kv4_first(w, U, W);
-    const long long run = kv4_first(w, runs, W);
-    if (run == runs) return U;
-    const int s = kv4_find(line.run0, p.c.n_seq, run);
-    return line.page0[s] + (run - line.run0[s]) * kv4_seq<PAIRS>(p, s).pages;
+  line.build<PAIRS>(p, piece_run + 2 * NW);
+  const int ctas = line.ctas(gridDim.x);
+  if ((int)blockIdx.x >= ctas) return;
+  const Kv4Split split(line.whole ? line.runs : line.U, ctas);
+  auto edge = [&](int c) {
+    const int x = split.first(c);
+    if (!line.whole) return x;
+    if (x == line.runs) return line.U;
+    const int s = line.find(line.run0, x);
+    return line.unit0[s] + (x - line.run0[s]) * kv4_seq<PAIRS>(p, s).units;
   };
-  const long long u0 = edge(worker), u1 = edge(worker + 1);
+  const int a0 = edge(blockIdx.x), a1 = edge(blockIdx.x + 1);
 
-  auto locate = [&](long long u) {
+  auto locate = [&](int u) {
     Kv4Unit x;
-    x.seq = kv4_find(line.page0, p.c.n_seq, u);
+    x.seq = line.find(line.unit0, u);
     x.q = kv4_seq<PAIRS>(p, x.seq);
-    const long long at = u - line.page0[x.seq], run = at / x.q.pages;
-    x.page = (int)(at - run * x.q.pages);
-    x.kv = (int)(run % p.c.n_kv);
-    x.tile = (int)(run / p.c.n_kv);
+    const int at = u - line.unit0[x.seq], run = at / x.q.units;
+    x.page = at - run * x.q.units - KV4_HEAD;
+    x.run = line.run0[x.seq] + run;
+    x.tile = run / p.c.n_kv;
+    x.kv = run - x.tile * p.c.n_kv;
     return x;
   };
-  // The page's K block, or null where there is nothing to see: no row of the
-  // tile reaches it, or the table names no page there.
-  auto find = [&](const Kv4Unit& x) -> const uint8_t* {
-    if (x.page * KV_PAGE > A::last_seen(x.q, x.tile, gqa)) return nullptr;
-    const int page = kv4_page(p.c, x.seq, x.page * KV_PAGE);
-    return page < 0 ? nullptr : kv4_block(p.c, page, x.kv, 0, A::BB);
+  // The K block of a run's page, or null where there is nothing to see: no row
+  // of the tile reaches it, or the table names no page there.
+  auto find = [&](int seq, int kv, int page, int seen) -> const uint8_t* {
+    if (page < 0 || page * KV_PAGE > seen) return nullptr;
+    const int at = kv4_page(p.c, seq, page * KV_PAGE);
+    return at < 0 ? nullptr : kv4_block(p.c, at, kv, 0, A::BB);
   };
   auto ask = [&](const uint8_t* block, int side) {  // the ring's K or V
     if (block && lane == 0) {
@@ -600,67 +659,118 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
   unsigned phase = 0;  // of both barriers
   bool dead = false;   // a wait gave up: the results are not valid, and nothing more is asked for
   auto arrived = [&](int side) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar + side, phase))) return;
     if (__any_sync(0xffffffffu, !mbar_wait(bar + side, phase))) {
       if (lane == 0 && p.c.err) atomicExch(p.c.err, KERR_WAIT);
       dead = true;
     }
   };
 
-  A w;
-  w.sums = reinterpret_cast<float4*>(smem + (size_t)NW * A::PAGE_BYTES) + warp * A::SUM_VECS * 32 + lane;
-  int since = 0;       // pages whose sums are in registers
-  Kv4Unit cur = locate(u0);
-  const uint8_t* block = find(cur);
-  ask(block, 0);
-  ask(block, 1);
-  w.template begin<T>(p, cur, gqa);
-  for (long long u = u0; u < u1; ++u) {
-    // the next page: its address is known before this one's codes are used up
-    Kv4Unit nxt = cur;
-    const bool last = u + 1 == u1;
-    if (++nxt.page == nxt.q.pages && !last) nxt = locate(u + 1);
-    const uint8_t* after = last || dead ? nullptr : find(nxt);
-    if (block) {
-      const int pos0 = cur.page * KV_PAGE;
-      arrived(0);
-      if (!dead) w.scores(ring);
-      __syncwarp();  // every lane has read K
-      if (!dead) ask(after, 0);
-      arrived(1);
-      if (!dead) {
-        if (pos0 + KV_PAGE - 1 > w.lim_min) w.template values<true>(ring + A::BB, pos0);
-        else w.template values<false>(ring + A::BB, pos0);
+  // the warp's stretch, behind the units that only stand ahead of a page
+  Kv4Unit cur = locate(a0);
+  const int from = a0 + min(max(0, -cur.page), min(a1 - a0, cur.q.units - KV4_HEAD - cur.page) - 1);  // of every run one is left
+  const Kv4Split mine(a1 - from, NW);
+  const int u0 = from + mine.first(warp), u1 = from + mine.first(warp + 1);
+  if (u0 < u1) {
+    A w;
+    w.sums = reinterpret_cast<float4*>(smem + (size_t)NW * A::PAGE_BYTES) + warp * A::SUM_VECS * 32 + lane;
+    int since = 0;  // pages whose sums are in registers
+    if (u0 != a0) cur = locate(u0);
+    int seq = cur.seq, kv = cur.kv, page = cur.page, end = cur.q.units - KV4_HEAD;
+    const uint8_t* block = find(seq, kv, page, A::last_seen(cur.q, cur.tile, gqa));
+    ask(block, 0);
+    ask(block, 1);
+    w.template begin<T>(p, cur, gqa);
+    for (int u = u0; u < u1; ++u) {
+      // the next page's address is known before this one's codes are used up
+      const uint8_t* after = nullptr;
+      const bool over = page + 1 == end, last = u + 1 == u1;  // the run's last unit, this warp's
+      if (!last && !dead) {
+        if (over) {
+          const Kv4Unit nxt = locate(u + 1);
+          after = find(nxt.seq, nxt.kv, nxt.page, A::last_seen(nxt.q, nxt.tile, gqa));
+        } else {
+          after = find(seq, kv, page + 1, w.lim_max);
+        }
       }
-      __syncwarp();
-      if (!dead) ask(after, 1);
-      phase ^= 1;
-      if (++since == KV4_FLUSH) { w.flush(); since = 0; }
-    } else {
-      ask(after, 0);
-      ask(after, 1);
+      if (block) {
+        const int pos0 = page * KV_PAGE;
+        arrived(0);
+        if (!dead) w.scores(ring);
+        __syncwarp();  // every lane has read K
+        if (!dead) ask(after, 0);
+        arrived(1);
+        if (!dead) {
+          if (pos0 + KV_PAGE - 1 > w.lim_min) w.template values<true>(ring + A::BB, pos0);
+          else w.template values<false>(ring + A::BB, pos0);
+        }
+        __syncwarp();
+        if (!dead) ask(after, 1);
+        phase ^= 1;
+        if (++since == KV4_FLUSH) { w.flush(); since = 0; }
+      } else {
+        ask(after, 0);
+        ask(after, 1);
+      }
+      block = dead ? nullptr : after;
+      ++page;
+      if (over || last) {
+        cur = locate(u);
+        const int run_first = u - (cur.page + KV4_HEAD);
+        const bool whole = over && (run_first >= u0 || (u0 == from && run_first >= a0));
+        float* part = last ? reinterpret_cast<float*>(ring) : p.heads + ((size_t)blockIdx.x * NW + warp) * (PAIRS * A::PART);
+        w.template end<T>(p, cur, gqa, whole ? nullptr : part);
+        if (!whole && lane == 0) piece_run[2 * warp + last] = cur.run;
+        if (!last) {
+          cur = locate(u + 1);
+          seq = cur.seq; kv = cur.kv; page = cur.page; end = cur.q.units - KV4_HEAD;
+          w.template begin<T>(p, cur, gqa);
+          since = 0;
+        }
+      }
     }
-    if (last || nxt.page == 0 || nxt.page == nxt.q.pages) {  // the run's end, or this worker's
-      const long long run_first = u - cur.page;
-      const bool whole = run_first >= u0 && cur.page + 1 == cur.q.pages;
-      float* part = p.part + ((size_t)worker * 2 + (run_first <= u0 ? 0 : 1)) * (PAIRS * A::PART);
-      w.template end<T>(p, cur, gqa, whole ? nullptr : part);
-      if (!last) w.template begin<T>(p, nxt, gqa);
-      since = 0;
-    }
-    cur = nxt;
-    block = dead ? nullptr : after;
   }
-  if (dead)  // copies in flight end before the CTA does
+  if (dead)  // copies in flight end before their memory is used for something else
     for (int i = 0; i < 4; ++i) mbar_wait(bar + i / 2, i & 1);
+  __syncthreads();
+
+  // the pieces of each run, in line: piece 2w is in the workspace, 2w + 1 in
+  // warp w's ring
+  for (int x = warp; x < 2 * NW * PAIRS; x += NW) {
+    const int k = x / PAIRS, i = x % PAIRS, run = piece_run[k];
+    if (run < 0) continue;
+    int before = k - 1;
+    while (before >= 0 && piece_run[before] < 0) --before;
+    if (before >= 0 && piece_run[before] == run) continue;  // joined with that one
+    const int s = line.find(line.run0, run);
+    const Kv4Seq q = kv4_seq<PAIRS>(p, s);
+    const int r = run - line.run0[s], kv = r % p.c.n_kv, pr = r / p.c.n_kv * PAIRS + i;
+    if (pr >= q.T * gqa) continue;
+    Kv4Sum<HD> sum;
+    for (int j = k; j < 2 * NW && (piece_run[j] < 0 || piece_run[j] == run); ++j) {
+      if (piece_run[j] < 0) continue;
+      sum.add((j & 1 ? reinterpret_cast<const float*>(smem + (size_t)(j / 2) * A::PAGE_BYTES)
+                     : p.heads + ((size_t)blockIdx.x * NW + j / 2) * (PAIRS * A::PART)) + i * A::PART);
+    }
+    const int first = line.unit0[s] + r * q.units;
+    if (first >= a0 && first + q.units <= a1) {
+      sum.store(static_cast<T*>(p.out) + ((size_t)(q.r0 + pr / gqa) * p.n_head + kv * gqa + pr % gqa) * HD);
+    } else {  // the end of a run that began earlier, or the beginning of one that goes on
+      float* dst = p.part + (((size_t)blockIdx.x * 2 + (first >= a0)) * PAIRS + i) * A::PART;
+      if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(sum.M, sum.l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) dst[4 + e * 32 + lane] = sum.v[e];
+    }
+  }
 }
 
-// Joins the pieces of split runs, in the line's order. A pair of a run takes
-// 1, 2, 4 or 8 of the CTA's warps, by how many pieces a run has on average;
-// each takes every such-th piece.
+// Joins the CTAs' pieces of split runs, in the line's order. A pair of a run
+// takes 1, 2, 4 or 8 of the CTA's warps, by how many pieces a run has on
+// average; each takes every such-th piece.
 constexpr int KV4_JOIN_WARPS = 8;
 template <int HD>
 __host__ __device__ constexpr int kv4_join_smem(int n_seq) {
-  return KV4_JOIN_WARPS * (HD + 2) * 4 + (n_seq + 1) * 16;
+  return KV4_JOIN_WARPS * (HD + 2) * 4 + Kv4Line::bytes(n_seq);
 }
 template <int HD, typename T, int NT>
 __global__ void __launch_bounds__(KV4_JOIN_WARPS * 32) kv4_join_kernel(const Kv4AttnParams p) {
@@ -669,63 +779,50 @@ __global__ void __launch_bounds__(KV4_JOIN_WARPS * 32) kv4_join_kernel(const Kv4
   extern __shared__ __align__(16) uint8_t smem[];
   float* red = reinterpret_cast<float*>(smem);  // [JW][HD + 2]
   Kv4Line line;
-  line.page0 = reinterpret_cast<long long*>(smem + JW * (HD + 2) * 4);
-  line.run0 = line.page0 + p.c.n_seq + 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gqa = p.n_head / p.c.n_kv;
-  kv4_line<PAIRS>(p, line);  // of arrays that the attention does not write
-  griddep_wait();            // by every thread: the end of this kernel stands for the end of the attention too
-  const long long U = line.page0[p.c.n_seq], pairs = line.run0[p.c.n_seq] * PAIRS;
-  if (U == 0) return;
-  const int W = kv4_workers(U, p.ctas, A::NW);
+  line.build<PAIRS>(p, red + JW * (HD + 2));  // of arrays that the attention does not write
+  griddep_wait();  // by every thread: the end of this kernel stands for the end of the attention too
+  const int ctas = line.ctas(p.ctas);
+  if (line.whole || ctas == 0) return;
+  const Kv4Split split(line.U, ctas);
   int team = 1;  // warps of a pair
-  while (team < JW && (long long)team * 8 * line.run0[p.c.n_seq] < W) team *= 2;
+  while (team < JW && team * 8 * line.runs < ctas) team *= 2;
   const int teams = JW / team, in_team = warp % team;
+  const long long pairs = (long long)line.runs * PAIRS;
   for (long long x0 = (long long)blockIdx.x * teams; x0 < pairs; x0 += (long long)gridDim.x * teams) {
-    const long long x = x0 + warp / team, run = x / PAIRS;
-    float l = 0.0f, sum[E] = {};
+    const long long x = x0 + warp / team;
+    const int run = (int)(x / PAIRS), i = (int)(x % PAIRS);
+    Kv4Sum<HD> sum;
     T* out = nullptr;
     if (x < pairs) {
-      const int i = (int)(x - run * PAIRS), s = kv4_find(line.run0, p.c.n_seq, run);
+      const int s = line.find(line.run0, run);
       const Kv4Seq q = kv4_seq<PAIRS>(p, s);
-      const int r = (int)(run - line.run0[s]), kv = r % p.c.n_kv, pr = r / p.c.n_kv * PAIRS + i;
-      const long long a = line.page0[s] + (long long)r * q.pages;
-      const int w0 = kv4_owner(a, U, W), w1 = kv4_owner(a + q.pages - 1, U, W);
-      if (w0 != w1 && pr < q.T * gqa) {
+      const int r = run - line.run0[s], kv = r % p.c.n_kv, pr = r / p.c.n_kv * PAIRS + i;
+      const int first = line.unit0[s] + r * q.units;
+      const int c0 = split.owner(first), c1 = split.owner(first + q.units - 1);
+      if (c0 != c1 && pr < q.T * gqa) {
         out = static_cast<T*>(p.out) + ((size_t)(q.r0 + pr / gqa) * p.n_head + kv * gqa + pr % gqa) * HD;
-        // a run's first piece may be the second of its worker; the others are their workers' first
-        const float* head = p.part + (((size_t)w0 * 2 + (a <= kv4_first(w0, U, W) ? 0 : 1)) * PAIRS + i) * A::PART;
-        auto piece = [&](int w) { return w == w0 ? head : p.part + ((size_t)w * 2 * PAIRS + i) * A::PART; };
-        float M = -INFINITY;
-        for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, *piece(w));
-        M = warp_max(M);
 #pragma unroll 4
-        for (int w = w0 + in_team; w <= w1; w += team) {
-          const float* src = piece(w);
-          const float2 ml = *reinterpret_cast<const float2*>(src);
-          // a piece that saw nothing counts for nothing
-          const float by = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : exp2_approx(ml.x - M);
-          l = fmaf(ml.y, by, l);
-#pragma unroll
-          for (int e = 0; e < E; ++e) sum[e] = fmaf(src[4 + e * 32 + lane], by, sum[e]);
-        }
+        for (int c = c0 + in_team; c <= c1; c += team)
+          sum.add(p.part + (((size_t)c * 2 + (c == c0)) * PAIRS + i) * A::PART);
       }
     }
     if (team > 1) {
       __syncthreads();  // red is free
 #pragma unroll
-      for (int e = 0; e < E; ++e) red[warp * (HD + 2) + e * 32 + lane] = sum[e];
-      if (lane == 0) red[warp * (HD + 2) + HD] = l;
+      for (int e = 0; e < E; ++e) red[warp * (HD + 2) + e * 32 + lane] = sum.v[e];
+      if (lane == 0) { red[warp * (HD + 2) + HD] = sum.M; red[warp * (HD + 2) + HD + 1] = sum.l; }
       __syncthreads();
       if (in_team) continue;
       for (int k = 1; k < team; ++k) {
-        l += red[(warp + k) * (HD + 2) + HD];
+        const float* from = red + (warp + k) * (HD + 2);
+        float v[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] += red[(warp + k) * (HD + 2) + e * 32 + lane];
+        for (int e = 0; e < E; ++e) v[e] = from[e * 32 + lane];
+        sum.add(from[HD], from[HD + 1], v);
       }
     }
-    if (out)
-#pragma unroll
-      for (int e = 0; e < E; ++e) out[e * 32 + lane] = (T)(l == 0.0f ? 0.0f : __fdiv_rn(sum[e], l));
+    if (out) sum.store(out);
   }
 }
 
