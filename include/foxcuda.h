@@ -229,9 +229,10 @@ foxcuda_status foxcuda_kv4_read(const foxcuda_kv4 *c, int ggml_type, void *k, vo
  * statistics are fp32. The same call gives the same bits; a row's sums are
  * split where an even division of the call's pages falls, so its last bits
  * can differ beside other sequences. workspace holds
- * foxcuda_kv4_attention_workspace() bytes (16-byte aligned; need not be
- * initialised) of the current device; calls that may run at the same time must not share it. */
-size_t         foxcuda_kv4_attention_workspace(uint32_t head_dim);
+ * foxcuda_kv4_attention_workspace() bytes of the current device (16-byte
+ * aligned; need not be initialised; NULL where that is 0, for block tables of
+ * up to 16 pages); calls that may run at the same time must not share it. */
+size_t         foxcuda_kv4_attention_workspace(uint32_t head_dim, uint32_t table_stride);
 foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4 *c, int ggml_type, const void *q, size_t q_stride,
                                      uint32_t n_head, float scale, void *workspace,
                                      size_t workspace_bytes, void *out, void *stream);

@@ -87,7 +87,7 @@ _PROTOS = {
     "foxcuda_kv4_block_bytes": (_sz, [C.c_uint32]),
     "foxcuda_kv4_write": (_st, [_vp, C.c_int, _vp, _sz, _vp, _sz, _vp]),
     "foxcuda_kv4_read": (_st, [_vp, C.c_int, _vp, _vp, _vp]),
-    "foxcuda_kv4_attention_workspace": (_sz, [C.c_uint32]),
+    "foxcuda_kv4_attention_workspace": (_sz, [C.c_uint32, C.c_uint32]),
     "foxcuda_kv4_attention": (_st, [_vp, C.c_int, _vp, _sz, C.c_uint32, C.c_float, _vp, _sz, _vp, _vp]),
     "foxcuda_qk_norm_rope": (_st, [C.c_int, _vp, _sz, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
                                    _vp, _vp, C.c_float, _vp, _vp, C.c_uint32, C.c_int, _vp, _vp, _sz,
@@ -361,76 +361,69 @@ def kv4_cache(n_pages: int, n_head_kv: int, head_dim: int, device="cuda"):
     return torch.zeros(n_pages, n_head_kv, 2, n, dtype=torch.uint8, device=device)
 
 
-def _row_type(t, what: str) -> int:
+def _bad(what: str, why: str, status: int = ERR_ARG):
+    raise FoxError(status, f"{what}: {why}")
+
+
+def _row_type(what: str, dtype) -> int:
     import torch
-    if t.dtype is torch.float32:
+    if dtype is torch.float32:
         return F.F32
-    if t.dtype is torch.float16:
+    if dtype is torch.float16:
         return F.F16
-    raise FoxError(ERR_UNSUPPORTED, f"{what}: rows of {t.dtype} are not covered (float32, float16)")
+    _bad(what, f"rows of {dtype} are not covered (float32, float16)", ERR_UNSUPPORTED)
 
 
-def _bad(what: str, why: str):
-    raise FoxError(ERR_ARG, f"{what}: {why}")
-
-
-def _same_device(what: str, t, *others):
-    if not t.is_cuda:
-        _bad(what, "the tensors must be on a CUDA device")
-    d = t.get_device()
-    for o in others:
-        if o is not None and o.get_device() != d:
-            _bad(what, "the tensors are on different devices")
-    return d
-
-
-def _call_on(device: int, fn, *args):
-    """fn(*args, stream) with `device` current, on its current stream."""
+def _call_on(what: str, fn, args, tensors):
+    """fn(*args, stream) on the device of the tensors (made current for the
+    call) and its current stream."""
     import torch
-    if device == torch.cuda.current_device():
-        _check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
+    d = tensors[0].get_device()
+    if d < 0:
+        _bad(what, "the tensors must be on a CUDA device")
+    for t in tensors:
+        if t is not None and t.get_device() != d:
+            _bad(what, "the tensors are on different devices")
+    if d == torch._C._cuda_getDevice():
+        _check(fn(*args, torch._C._cuda_getCurrentRawStream(d)))
     else:
-        with torch.cuda.device(device):
-            _check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
+        with torch.cuda.device(d):
+            _check(fn(*args, torch._C._cuda_getCurrentRawStream(d)))
 
 
 def _kv4(what: str, cache, table, row_start, kv_len, n_rows: int):
     import torch
-    if cache.dtype is not torch.uint8 or cache.dim() != 4 or cache.shape[2] != 2 or not cache.is_contiguous():
+    i32, shape = torch.int32, cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 4 or shape[2] != 2 or not cache.is_contiguous():
         _bad(what, "the cache is a contiguous uint8 tensor [pages, kv heads, 2, block] (kv4_cache)")
-    n_pages, n_kv, _, block = cache.shape
-    i32 = torch.int32
-    if table.dtype is not i32 or table.dim() != 2 or not table.is_contiguous():
-        _bad(what, "table is a contiguous int32 tensor [sequences, pages]")
-    n_seq, stride = table.shape
-    if kv_len.dtype is not i32 or kv_len.dim() != 1 or not kv_len.is_contiguous() or kv_len.shape[0] != n_seq:
-        _bad(what, f"kv_len is a contiguous int32 tensor of {n_seq} lengths")
-    if (row_start.dtype is not i32 or row_start.dim() != 1 or not row_start.is_contiguous()
-            or row_start.shape[0] != n_seq + 1):
-        _bad(what, f"row_start is a contiguous int32 tensor of {n_seq + 1} rows")
-    hd = block // KV4_BLOCK_PER_DIM
-    if hd * KV4_BLOCK_PER_DIM != block:
+    n_pages, n_kv, _, block = shape
+    hd, rest = divmod(block, KV4_BLOCK_PER_DIM)
+    if rest:
         _bad(what, f"blocks of {block} bytes belong to no head dimension")
+    shape = table.shape
+    if table.dtype is not i32 or len(shape) != 2 or not table.is_contiguous():
+        _bad(what, "table is a contiguous int32 tensor [sequences, pages]")
+    n_seq, stride = shape
+    if kv_len.dtype is not i32 or kv_len.shape != (n_seq,) or not kv_len.is_contiguous():
+        _bad(what, f"kv_len is a contiguous int32 tensor of {n_seq} lengths")
+    if row_start.dtype is not i32 or row_start.shape != (n_seq + 1,) or not row_start.is_contiguous():
+        _bad(what, f"row_start is a contiguous int32 tensor of {n_seq + 1} rows")
     return Kv4(cache.data_ptr(), table.data_ptr(), row_start.data_ptr(), kv_len.data_ptr(), n_pages, n_kv, hd,
                n_seq, stride, n_rows)
 
 
-def _rows(what: str, name: str, t, heads: int, hd: int):
-    """t as rows of heads * hd values ([rows, heads * hd] or [rows, heads, hd],
-    each row contiguous): its row stride in elements."""
+def _rows(what: str, name: str, t, n_rows: int, heads: int, hd: int, dtype) -> int:
+    """t as n_rows rows of heads * hd values ([rows, heads * hd] or [rows,
+    heads, hd], each row contiguous): its row stride in elements."""
     shape, stride = t.shape, t.stride()
     if len(shape) == 2:
         ok = shape[1] == heads * hd and stride[1] == 1
     else:
         ok = len(shape) == 3 and shape[1] == heads and shape[2] == hd and stride[2] == 1 and (heads == 1 or stride[1] == hd)
-    if not ok:
-        _bad(what, f"{name} holds rows of {heads} x {hd} values, each row contiguous; got {tuple(shape)}")
-    return stride[0] if shape[0] > 1 else max(stride[0], heads * hd)
-
-
-def _contiguous_rows(what: str, name: str, t, n_rows: int, heads: int, hd: int, like):
-    if t.dtype is not like or not t.is_contiguous() or t.numel() != n_rows * heads * hd or t.shape[0] != n_rows:
-        _bad(what, f"{name} is a contiguous {like} tensor of {n_rows} rows of {heads} x {hd} values")
+    if not ok or shape[0] != n_rows or t.dtype is not dtype:
+        _bad(what, f"{name} holds {n_rows} {dtype} rows of {heads} x {hd} values, each row contiguous; "
+                   f"got {t.dtype} {tuple(shape)}")
+    return stride[0] if n_rows > 1 else max(stride[0], heads * hd)
 
 
 def kv4_write(cache, table, row_start, kv_len, k, v):
@@ -438,13 +431,13 @@ def kv4_write(cache, table, row_start, kv_len, k, v):
     (foxcuda_kv4_write). Sequence s has the rows row_start[s] ..
     row_start[s+1]-1, which stand at the last of its kv_len[s] positions;
     page table[s, p // 64] holds position p."""
-    c = _kv4("kv4_write", cache, table, row_start, kv_len, k.shape[0])
-    if k.dtype is not v.dtype or v.shape[0] != k.shape[0]:
-        _bad("kv4_write", "k and v have the same rows and type")
-    ks = _rows("kv4_write", "k", k, c.n_head_kv, c.head_dim)
-    vs = _rows("kv4_write", "v", v, c.n_head_kv, c.head_dim)
-    d = _same_device("kv4_write", cache, table, row_start, kv_len, k, v)
-    _call_on(d, lib().foxcuda_kv4_write, C.byref(c), _row_type(k, "kv4_write"), k.data_ptr(), ks, v.data_ptr(), vs)
+    what, n, dtype = "kv4_write", k.shape[0], k.dtype
+    c = _kv4(what, cache, table, row_start, kv_len, n)
+    ks = _rows(what, "k", k, n, c.n_head_kv, c.head_dim, dtype)
+    vs = _rows(what, "v", v, n, c.n_head_kv, c.head_dim, dtype)
+    _call_on(what, lib().foxcuda_kv4_write,
+             (C.byref(c), _row_type(what, dtype), k.data_ptr(), ks, v.data_ptr(), vs),
+             (cache, table, row_start, kv_len, k, v))
 
 
 def kv4_read(cache, table, row_start, kv_len, n_rows: int | None = None, dtype=None, k_out=None, v_out=None):
@@ -453,17 +446,20 @@ def kv4_read(cache, table, row_start, kv_len, n_rows: int | None = None, dtype=N
     v_out, or into new tensors of `dtype` (float32) where padding rows are
     zeros."""
     import torch
+    what = "kv4_read"
     if (k_out is None) != (v_out is None) or (k_out is None and n_rows is None):
-        _bad("kv4_read", "give both k_out and v_out, or n_rows")
+        _bad(what, "give both k_out and v_out, or n_rows")
     n = k_out.shape[0] if k_out is not None else n_rows
-    c = _kv4("kv4_read", cache, table, row_start, kv_len, n)
+    c = _kv4(what, cache, table, row_start, kv_len, n)
+    hd, kv = c.head_dim, c.n_head_kv
     if k_out is None:
-        dtype = dtype or torch.float32
-        k_out, v_out = (torch.zeros(n, c.n_head_kv, c.head_dim, dtype=dtype, device=cache.device) for _ in "kv")
+        k_out, v_out = (torch.zeros(n, kv, hd, dtype=dtype or torch.float32, device=cache.device) for _ in "kv")
+    dtype = k_out.dtype
     for name, x in (("k_out", k_out), ("v_out", v_out)):
-        _contiguous_rows("kv4_read", name, x, n, c.n_head_kv, c.head_dim, k_out.dtype)
-    d = _same_device("kv4_read", cache, table, row_start, kv_len, k_out, v_out)
-    _call_on(d, lib().foxcuda_kv4_read, C.byref(c), _row_type(k_out, "kv4_read"), k_out.data_ptr(), v_out.data_ptr())
+        if _rows(what, name, x, n, kv, hd, dtype) != kv * hd:
+            _bad(what, f"{name} must be contiguous")
+    _call_on(what, lib().foxcuda_kv4_read, (C.byref(c), _row_type(what, dtype), k_out.data_ptr(), v_out.data_ptr()),
+             (cache, table, row_start, kv_len, k_out, v_out))
     return k_out, v_out
 
 
@@ -474,33 +470,41 @@ def kv4_attention(q, cache, table, row_start, kv_len, scale: float = 0.0, out=No
     uint8 tensor of kv4_attention_workspace() bytes to use instead of a new
     one; calls that may run at the same time must not share it."""
     import torch
-    n, what = q.shape[0], "kv4_attention"
+    what, n, dtype = "kv4_attention", q.shape[0], q.dtype
     c = _kv4(what, cache, table, row_start, kv_len, n)
-    heads = q.shape[1] if q.dim() == 3 else q.shape[1] // c.head_dim
-    qs = _rows(what, "q", q, heads, c.head_dim)
+    hd = c.head_dim
+    heads = q.shape[1] if q.dim() == 3 else q.shape[1] // max(hd, 1)
+    qs = _rows(what, "q", q, n, heads, hd, dtype)
     if out is None:
-        out = torch.zeros(n, heads, c.head_dim, dtype=q.dtype, device=q.device)
-    else:
-        _contiguous_rows(what, "out", out, n, heads, c.head_dim, q.dtype)
-    L = lib()
-    d = _same_device(what, cache, table, row_start, kv_len, q, out, workspace)
-    if workspace is None:
-        workspace = torch.empty(kv4_attention_workspace(c.head_dim, d), dtype=torch.uint8,
-                                device=q.device)
-    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
-        _bad(what, "workspace is a contiguous uint8 tensor")
-    _call_on(d, L.foxcuda_kv4_attention, C.byref(c), _row_type(q, what), q.data_ptr(), qs, heads, scale,
-             workspace.data_ptr(), workspace.numel(), out.data_ptr())
+        out = torch.zeros(n, heads, hd, dtype=dtype, device=q.device)
+    elif _rows(what, "out", out, n, heads, hd, dtype) != heads * hd:
+        _bad(what, "out must be contiguous")
+    size = 0
+    if workspace is not None:
+        if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+            _bad(what, "workspace is a contiguous uint8 tensor")
+        size = workspace.numel()
+    elif c.table_stride > KV4_WHOLE_PAGES:
+        size = kv4_attention_workspace(hd, c.table_stride, q.get_device())
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _call_on(what, lib().foxcuda_kv4_attention,
+             (C.byref(c), _row_type(what, dtype), q.data_ptr(), qs, heads, scale,
+              None if workspace is None else workspace.data_ptr(), size, out.data_ptr()),
+             (cache, table, row_start, kv_len, q, out, workspace))
     return out
 
 
-def kv4_attention_workspace(head_dim: int, device: int | None = None) -> int:
-    """Bytes of kv4_attention's workspace (on `device`, or the current one)."""
+KV4_WHOLE_PAGES = 16  # block tables of up to so many pages need no workspace
+
+
+def kv4_attention_workspace(head_dim: int, table_pages: int, device: int | None = None) -> int:
+    """Bytes of kv4_attention's workspace for block tables of table_pages
+    pages a sequence (on `device`, or the current one)."""
     import torch
-    if device is None or device == torch.cuda.current_device():
-        return lib().foxcuda_kv4_attention_workspace(head_dim)
+    if device is None or device < 0 or device == torch._C._cuda_getDevice():
+        return lib().foxcuda_kv4_attention_workspace(head_dim, table_pages)
     with torch.cuda.device(device):
-        return lib().foxcuda_kv4_attention_workspace(head_dim)
+        return lib().foxcuda_kv4_attention_workspace(head_dim, table_pages)
 
 
 def qk_norm_rope(x, n_head: int, n_head_kv: int, head_dim: int, pos, cos, sin, q_norm=None, k_norm=None,
@@ -513,32 +517,31 @@ def qk_norm_rope(x, n_head: int, n_head_kv: int, head_dim: int, pos, cos, sin, q
     k_out (which may be x's own rows), or new tensors where rows with a
     negative position are zeros."""
     import torch
-    what, n = "qk_norm_rope", x.shape[0]
-    nq, nk = n_head * head_dim, n_head_kv * head_dim
-    if x.dim() != 2 or x.shape[1] < nq + nk or (x.shape[1] > 1 and x.stride(1) != 1):
+    what, f32, shape, stride, dtype = "qk_norm_rope", torch.float32, x.shape, x.stride(), x.dtype
+    n, nq, nk = shape[0], n_head * head_dim, n_head_kv * head_dim
+    if len(shape) != 2 or shape[1] < nq + nk or stride[1] != 1:
         _bad(what, f"x holds rows of at least {nq + nk} values, each row contiguous")
     if q_out is None:
-        q_out = torch.zeros(n, n_head, head_dim, dtype=x.dtype, device=x.device)
+        q_out = torch.zeros(n, n_head, head_dim, dtype=dtype, device=x.device)
     if k_out is None:
-        k_out = torch.zeros(n, n_head_kv, head_dim, dtype=x.dtype, device=x.device)
-    qs, ks = _rows(what, "q_out", q_out, n_head, head_dim), _rows(what, "k_out", k_out, n_head_kv, head_dim)
-    if q_out.shape[0] != n or k_out.shape[0] != n or q_out.dtype is not x.dtype or k_out.dtype is not x.dtype:
-        _bad(what, "x, q_out and k_out have the same rows and type")
+        k_out = torch.zeros(n, n_head_kv, head_dim, dtype=dtype, device=x.device)
+    qs = _rows(what, "q_out", q_out, n, n_head, head_dim, dtype)
+    ks = _rows(what, "k_out", k_out, n, n_head_kv, head_dim, dtype)
     if pos.dtype is not torch.int32 or pos.shape != (n,) or not pos.is_contiguous():
         _bad(what, f"pos is a contiguous int32 tensor of {n} positions")
-    f32 = torch.float32
-    if (cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] * 2 != head_dim or cos.dtype is not f32
-            or sin.dtype is not f32 or not cos.is_contiguous() or not sin.is_contiguous()):
-        _bad(what, f"cos and sin are contiguous float32 tensors [positions, {head_dim // 2}]")
+    n_pos = cos.shape[0] if cos.dim() == 2 else 0
+    for t in (cos, sin):
+        if t.dtype is not f32 or t.shape != (n_pos, head_dim // 2) or not t.is_contiguous():
+            _bad(what, f"cos and sin are contiguous float32 tensors [positions, {head_dim // 2}]")
     for w in (q_norm, k_norm):
         if w is not None and (w.dtype is not f32 or w.shape != (head_dim,) or not w.is_contiguous()):
             _bad(what, f"the norm weights are contiguous float32 tensors of {head_dim} values")
-    d = _same_device(what, x, pos, cos, sin, q_norm, k_norm, q_out, k_out)
-    xs = x.stride(0) if n > 1 else max(x.stride(0), nq + nk)
-    _call_on(d, lib().foxcuda_qk_norm_rope, _row_type(x, what), x.data_ptr(), xs, n, n_head, n_head_kv, head_dim,
-             None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-             cos.data_ptr(), sin.data_ptr(), cos.shape[0], int(halves), pos.data_ptr(), q_out.data_ptr(), qs,
-             k_out.data_ptr(), ks)
+    _call_on(what, lib().foxcuda_qk_norm_rope,
+             (_row_type(what, dtype), x.data_ptr(), stride[0] if n > 1 else max(stride[0], nq + nk), n, n_head,
+              n_head_kv, head_dim, None if q_norm is None else q_norm.data_ptr(),
+              None if k_norm is None else k_norm.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), n_pos, halves,
+              pos.data_ptr(), q_out.data_ptr(), qs, k_out.data_ptr(), ks),
+             (x, pos, cos, sin, q_norm, k_norm, q_out, k_out))
     return q_out, k_out
 
 

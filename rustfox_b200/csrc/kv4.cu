@@ -131,18 +131,14 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
   return FOXCUDA_OK;
 }
 
-// A tile's pieces: two of every CTA, and one of every warp.
-template <int HD, int NT>
-static size_t kv4_piece_floats(int ctas, int each) {
-  using A = Kv4Attn<HD, NT>;
-  return (size_t)ctas * each * A::PAIRS * A::PART;
-}
+// Two pieces of a tile for every CTA.
 template <int HD, int NT>
 static size_t kv4_work_bytes(int ctas) {
-  return kv4_piece_floats<HD, NT>(ctas, 2 + Kv4Attn<HD, NT>::NW) * 4;
+  return (size_t)ctas * 2 * Kv4Attn<HD, NT>::PIECE_BYTES;
 }
 
-extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim) {
+extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim, uint32_t table_stride) {
+  if (table_stride <= KV4_WHOLE) return 0;  // no run is split between CTAs
   const int ctas = current_sms();
   switch (head_dim) {
     case 64: return kv4_work_bytes<64, 1>(ctas);
@@ -153,9 +149,8 @@ extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim) {
 }
 
 template <typename T, int HD, int NT>
-static cudaError_t launch_kv4_attend(Kv4AttnParams p, cudaStream_t s) {
+static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
   using A = Kv4Attn<HD, NT>;
-  p.heads = p.part + kv4_piece_floats<HD, NT>(p.ctas, 2);
   const size_t smem = A::smem_bytes(p.c.n_seq);
   static size_t marks[kMaxDevices] = {}, join_marks[kMaxDevices] = {};
   cudaError_t e = opt_in_smem(kv4_attend_kernel<HD, T, NT>, smem, marks);
@@ -192,7 +187,8 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
     return fail(FOXCUDA_ERR_UNSUPPORTED, "kv4_attention: %u heads over %u KV heads are not covered", n_head, c->n_head_kv);
   if (!(scale >= 0.0f) || scale > 3.0e38f) return fail(FOXCUDA_ERR_ARG, "kv4_attention: scale %g", (double)scale);
   if (none) return FOXCUDA_OK;
-  if (!q || !out || !workspace) return fail(FOXCUDA_ERR_ARG, "kv4_attention: null pointer");
+  const size_t need = foxcuda_kv4_attention_workspace(c->head_dim, c->table_stride);
+  if (!q || !out || (need && !workspace)) return fail(FOXCUDA_ERR_ARG, "kv4_attention: null pointer");
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) ||
       !stride_ok(q_stride, (size_t)n_head * c->head_dim, type))
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: rows and workspace must be 16-byte aligned, rows at least a row apart");
@@ -201,7 +197,6 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
   if (units >= 2147483648.0)
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: %u rows over %u pages a sequence are too many for one call",
                 c->n_rows, c->table_stride);
-  const size_t need = foxcuda_kv4_attention_workspace(c->head_dim);
   if (workspace_bytes < need)
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: the workspace holds %zu bytes, %zu are needed", workspace_bytes, need);
   p.q = q; p.out = out; p.part = static_cast<float*>(workspace); p.q_stride = q_stride;

@@ -43,7 +43,7 @@ struct Kv4AttnParams {
   Kv4Rows c;
   const void* q;
   void* out;
-  float *part, *heads;  // workspace: pieces of runs split over CTAs, and over a CTA's warps
+  float* part;          // workspace: pieces of runs split between CTAs
   size_t q_stride;      // elements between rows
   int n_head, ctas;
   float scale;
@@ -256,10 +256,13 @@ struct Kv4Attn {
   static constexpr int PAIRS = 4 * NT;       // (row, head) pairs of a tile
   static constexpr int SUM_VECS = NT * SLABS * NB * 2;  // float4s of a lane's sums
   static constexpr int PART = HD + 4;        // floats of one pair's partial result: M, l, -, -, sums
-  // warps of a CTA, each with room for a page's K and V: what the registers hold
-  static constexpr int NW = HD < 256 ? 12 : 8;
+  // warps of a CTA: what the registers (and for 256 dimensions shared memory)
+  // hold. Each has room for a page's K and V, then for a piece of a run; for
+  // its flushed sums; and for the piece it may end before that.
+  static constexpr int NW = HD < 256 ? 12 : 7, PIECE_BYTES = PAIRS * PART * 4;
+  static_assert(PIECE_BYTES <= PAGE_BYTES && PIECE_BYTES % 16 == 0, "a piece fits the ring");
   static constexpr size_t smem_bytes(int n_seq) {
-    return (size_t)NW * (PAGE_BYTES + SUM_VECS * 512) + NW * 2 * 8 + NW * 2 * 4 + Kv4Line::bytes(n_seq);
+    return (size_t)NW * (PAGE_BYTES + SUM_VECS * 512 + PIECE_BYTES) + NW * 2 * 8 + NW * 2 * 4 + Kv4Line::bytes(n_seq);
   }
 
   // A warp's share of a tile: q's operand registers, and the running maximum,
@@ -604,7 +607,8 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint8_t* ring = smem + (size_t)warp * A::PAGE_BYTES;
-  uint8_t* behind = smem + (size_t)NW * (A::PAGE_BYTES + A::SUM_VECS * 512);
+  uint8_t* heads = smem + (size_t)NW * (A::PAGE_BYTES + A::SUM_VECS * 512);
+  uint8_t* behind = heads + (size_t)NW * A::PIECE_BYTES;
   uint64_t* bar = reinterpret_cast<uint64_t*>(behind) + warp * 2;
   int* piece_run = reinterpret_cast<int*>(behind + NW * 2 * 8);  // [2 NW], in line: the runs of the warps' pieces, or -1
   Kv4Line line;
@@ -718,7 +722,7 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
         cur = locate(u);
         const int run_first = u - (cur.page + KV4_HEAD);
         const bool whole = over && (run_first >= u0 || (u0 == from && run_first >= a0));
-        float* part = last ? reinterpret_cast<float*>(ring) : p.heads + ((size_t)blockIdx.x * NW + warp) * (PAIRS * A::PART);
+        float* part = reinterpret_cast<float*>(last ? ring : heads + (size_t)warp * A::PIECE_BYTES);
         w.template end<T>(p, cur, gqa, whole ? nullptr : part);
         if (!whole && lane == 0) piece_run[2 * warp + last] = cur.run;
         if (!last) {
@@ -734,8 +738,8 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
     for (int i = 0; i < 4; ++i) mbar_wait(bar + i / 2, i & 1);
   __syncthreads();
 
-  // the pieces of each run, in line: piece 2w is in the workspace, 2w + 1 in
-  // warp w's ring
+  // the pieces of each run, in line: piece 2w is one that warp w ended before
+  // its last, which is 2w + 1 and in its ring
   for (int x = warp; x < 2 * NW * PAIRS; x += NW) {
     const int k = x / PAIRS, i = x % PAIRS, run = piece_run[k];
     if (run < 0) continue;
@@ -749,8 +753,8 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
     Kv4Sum<HD> sum;
     for (int j = k; j < 2 * NW && (piece_run[j] < 0 || piece_run[j] == run); ++j) {
       if (piece_run[j] < 0) continue;
-      sum.add((j & 1 ? reinterpret_cast<const float*>(smem + (size_t)(j / 2) * A::PAGE_BYTES)
-                     : p.heads + ((size_t)blockIdx.x * NW + j / 2) * (PAIRS * A::PART)) + i * A::PART);
+      sum.add(reinterpret_cast<const float*>(j & 1 ? smem + (size_t)(j / 2) * A::PAGE_BYTES
+                                                   : heads + (size_t)(j / 2) * A::PIECE_BYTES) + i * A::PART);
     }
     const int first = line.unit0[s] + r * q.units;
     if (first >= a0 && first + q.units <= a1) {

@@ -94,6 +94,8 @@ def test_every_call_refuses_a_bad_cache(buf, change, want):
 def test_rows_types_and_strides_are_refused(buf):
     rf, L = _lib()
     c = C.byref(_view(rf, buf))
+    w = C.byref(_view(rf, buf, table_stride=17))
+    huge = C.byref(_view(rf, buf, n_rows=1 << 20, table_stride=1 << 12))  # 2^31 pages of tiles
     odd = buf + 8
     cases = [
         (L.foxcuda_kv4_write(None, 0, buf, 128, buf, 128, None), 1),
@@ -111,14 +113,17 @@ def test_rows_types_and_strides_are_refused(buf):
         (L.foxcuda_kv4_attention(c, 0, buf, 256, 4, -1.0, buf, 1 << 40, buf, None), 1),
         (L.foxcuda_kv4_attention(c, 0, buf, 256, 4, float("nan"), buf, 1 << 40, buf, None), 1),
         (L.foxcuda_kv4_attention(c, 0, buf, 256, 4, float("inf"), buf, 1 << 40, buf, None), 1),
-        (L.foxcuda_kv4_attention(c, 0, buf, 256, 4, 0.0, buf, 16, buf, None), 1),         # workspace too small
-        (L.foxcuda_kv4_attention(c, 0, buf, 256, 4, 0.0, None, 1 << 40, buf, None), 1),
+        (L.foxcuda_kv4_attention(w, 0, buf, 256, 4, 0.0, buf, 16, buf, None), 1),         # workspace too small
+        (L.foxcuda_kv4_attention(w, 0, buf, 256, 4, 0.0, None, 1 << 40, buf, None), 1),
+        (L.foxcuda_kv4_attention(huge, 0, buf, 256, 4, 0.0, buf, 1 << 40, buf, None), 1),
         (L.foxcuda_kv4_attention(c, 0, buf, 256, 4, 0.0, buf, 1 << 40, odd, None), 1),
     ]
     for i, (got, want) in enumerate(cases):
         assert got == want, i
     assert L.foxcuda_kv4_block_bytes(96) == 0 and L.foxcuda_kv4_block_bytes(128) == R.block_bytes(128)
-    assert L.foxcuda_kv4_attention_workspace(96) == 0
+    assert L.foxcuda_kv4_attention_workspace(96, 100) == 0
+    assert L.foxcuda_kv4_attention_workspace(128, 16) == 0 < L.foxcuda_kv4_attention_workspace(128, 17)
+    assert rf.api.KV4_WHOLE_PAGES == 16
 
 
 def test_a_call_without_rows_or_sequences_does_nothing(buf):

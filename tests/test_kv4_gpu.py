@@ -516,10 +516,10 @@ def test_a_captured_step_follows_its_device_lengths():
     heads, kv, hd, n_seq = 8, 2, 128, 3
     sets = []
     for k in range(2):
-        st, rng = _setup(heads, kv, hd, n_seq, 8, n_seq, seed=20 + k)
-        st.update(lens=i32([500 - 100 * k, 3, 64]), x=torch.empty(n_seq, (heads + 2 * kv) * hd, device=DEV),
+        st, rng = _setup(heads, kv, hd, n_seq, 20, n_seq, seed=20 + k)
+        st.update(lens=i32([1200 - 100 * k, 3, 64]), x=torch.empty(n_seq, (heads + 2 * kv) * hd, device=DEV),
                   start=i32(range(n_seq + 1)), seed=k, eager=st["cache"].clone(),
-                  work=torch.empty(rf.kv4_attention_workspace(hd), dtype=torch.uint8, device=DEV))
+                  work=torch.empty(rf.kv4_attention_workspace(hd, 20), dtype=torch.uint8, device=DEV))
         st["cache"].random_(0, 60), st["eager"].copy_(st["cache"])  # finite parameters
         sets.append(st)
     rf.kernel_errors()
