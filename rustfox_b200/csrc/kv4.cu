@@ -63,9 +63,20 @@ static cudaError_t by_type_hd(int type, uint32_t hd, F f) {
   return type == T_F32 ? with(float()) : with(__half());
 }
 
+// One pass a warp where the rows are few, so that they spread over the device;
+// four, for one search for the row's place, where they fill it anyway.
+template <int HD, typename F>
+static cudaError_t by_batch(const Kv4Rows& c, F f) {
+  const int passes = Kv4Pass<HD>::passes(c.n_kv);
+  const auto grid = [&](int batch) { return (unsigned)(((size_t)c.n_rows * ((passes + batch - 1) / batch) + 7) / 8); };
+  if ((long long)c.n_rows * passes > 32LL * current_sms()) f(std::integral_constant<int, 4>(), grid(4));
+  else f(std::integral_constant<int, 1>(), grid(1));
+  return cudaGetLastError();
+}
+
 extern "C" foxcuda_status foxcuda_kv4_write(const foxcuda_kv4* c, int type, const void* k, size_t k_stride,
                                             const void* v, size_t v_stride, void* stream) {
-  Kv4WriteParams p{};
+  Kv4MoveParams p{};
   bool none = false;
   foxcuda_status st = check_kv4(c, type, "kv4_write", &p.c, &none);
   if (st || none) return st;
@@ -73,29 +84,44 @@ extern "C" foxcuda_status foxcuda_kv4_write(const foxcuda_kv4* c, int type, cons
   if (!k || !v) return fail(FOXCUDA_ERR_ARG, "kv4_write: null pointer");
   if (!aligned16(k) || !aligned16(v) || !stride_ok(k_stride, row, type) || !stride_ok(v_stride, row, type))
     return fail(FOXCUDA_ERR_ARG, "kv4_write: rows must be 16-byte aligned and at least a row apart");
-  p.k = k; p.v = v; p.k_stride = k_stride; p.v_stride = v_stride;
-  const size_t units = (size_t)c->n_rows * c->n_head_kv;
+  p.k = const_cast<void*>(k); p.v = const_cast<void*>(v); p.k_stride = k_stride; p.v_stride = v_stride;
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
-       kv4_write_kernel<decltype(tag), hd.value><<<(unsigned)((units + 7) / 8), 256, 0, (cudaStream_t)stream>>>(p);
-       return cudaGetLastError();
+       return by_batch<hd.value>(p.c, [&](auto batch, unsigned grid) {
+         kv4_write_kernel<decltype(tag), hd.value, batch.value><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+       });
      }), "kv4_write launch");
   return FOXCUDA_OK;
 }
 
 extern "C" foxcuda_status foxcuda_kv4_read(const foxcuda_kv4* c, int type, void* k, void* v, void* stream) {
-  Kv4ReadParams p{};
+  Kv4MoveParams p{};
   bool none = false;
   foxcuda_status st = check_kv4(c, type, "kv4_read", &p.c, &none);
   if (st || none) return st;
   if (!k || !v) return fail(FOXCUDA_ERR_ARG, "kv4_read: null pointer");
   if (!aligned16(k) || !aligned16(v)) return fail(FOXCUDA_ERR_ARG, "kv4_read: rows must be 16-byte aligned");
   p.k = k; p.v = v;
-  const size_t units = (size_t)c->n_rows * c->n_head_kv;
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
-       kv4_read_kernel<decltype(tag), hd.value><<<(unsigned)((units + 7) / 8), 256, 0, (cudaStream_t)stream>>>(p);
-       return cudaGetLastError();
+       return by_batch<hd.value>(p.c, [&](auto batch, unsigned grid) {
+         kv4_read_kernel<decltype(tag), hd.value, batch.value><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+       });
      }), "kv4_read launch");
   return FOXCUDA_OK;
+}
+
+template <typename T, int HD, bool HALVES, int BATCH>
+static cudaError_t launch_rope_b(const RopeParams& p, cudaStream_t s) {
+  using Y = RopeLay<T, HD>;
+  const size_t warps = (size_t)p.n_rows * (Y::chunks(p.n_head, BATCH) + Y::chunks(p.n_kv, BATCH));
+  qk_norm_rope_kernel<T, HD, HALVES, BATCH><<<(unsigned)((warps + 7) / 8), 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+// One load a warp where the rows are few, so that they spread over the device;
+// four, each row's tables loaded once for them, where they fill it anyway.
+template <typename T, int HD, bool HALVES>
+static cudaError_t launch_rope(const RopeParams& p, cudaStream_t s) {
+  const long long bytes = (long long)p.n_rows * (p.n_head + p.n_kv) * HD * sizeof(T);
+  return bytes > 512LL * 16 * current_sms() ? launch_rope_b<T, HD, HALVES, 4>(p, s) : launch_rope_b<T, HD, HALVES, 1>(p, s);
 }
 
 extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x_stride, uint32_t n_rows,
@@ -123,10 +149,9 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
   p.x_stride = x_stride; p.q_stride = q_stride; p.k_stride = k_stride;
   p.n_rows = (int)n_rows; p.n_head = (int)n_head; p.n_kv = (int)n_head_kv; p.n_pos = (int)n_pos; p.halves = halves;
   p.eps = eps; p.err = kernel_err_ptr();
-  const size_t units = (size_t)n_rows * (n_head + n_head_kv);
   CK(by_type_hd(type, head_dim, [&](auto tag, auto hd) {
-       qk_norm_rope_kernel<decltype(tag), hd.value><<<(unsigned)((units + 7) / 8), 256, 0, (cudaStream_t)stream>>>(p);
-       return cudaGetLastError();
+       return halves ? launch_rope<decltype(tag), hd.value, true>(p, (cudaStream_t)stream)
+                     : launch_rope<decltype(tag), hd.value, false>(p, (cudaStream_t)stream);
      }), "qk_norm_rope launch");
   return FOXCUDA_OK;
 }

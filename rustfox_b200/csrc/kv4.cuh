@@ -35,23 +35,6 @@ constexpr int KV4_GROUP = 64;
 __host__ __device__ constexpr int kv4_block_bytes(int hd) { return KV_PAGE * (hd / 2 + 4 * (hd / KV4_GROUP)); }
 __host__ __device__ constexpr int kv4_codes_bytes(int hd) { return KV_PAGE * hd / 2; }
 
-// Byte of the 16 bits that hold dimensions d..d+3 (d a multiple of 4) of
-// position p in a block.
-template <int HD>
-FOX_DEV int kv4_k_at(int p, int d) {
-  constexpr int SLAB = HD < 128 ? HD : 128, G = SLAB / 64;
-  const int r = d % SLAB;
-  return (d / SLAB) * (KV_PAGE * SLAB / 2) + p * (SLAB / 2) +
-         4 * ((r % 64 / 16) * 2 * G + 2 * (r / 64) + (r % 16) / 8) + (r % 8) / 2;
-}
-template <int HD>
-FOX_DEV int kv4_v_at(int p, int d) {
-  constexpr int SLAB = HD < 128 ? HD : 128, NB = SLAB / 32;
-  const int r = d % SLAB;
-  const int at = ((((d / SLAB) * 4 + p / 16) * 2 + (p / 8) % 2) * 4 + (p % 8) / 2) * 8 + (r % 32) / 4;
-  return 4 * (at * NB + r / 32) + 2 * (p % 2);
-}
-
 // Rows of sequences: sequence s has the rows row_start[s] ..
 // row_start[s+1]-1, standing at the last of its kv_len[s] cached positions.
 struct Kv4Rows {
@@ -62,19 +45,6 @@ struct Kv4Rows {
   int n_pages, n_kv, n_seq, table_stride, n_rows;
   int* err;
 };
-
-// The sequence of a row (all lanes of a warp ask for the same row): the
-// number of sequences that end at or before it. One round of loads for every
-// 32 sequences. n_seq for a padding row.
-FOX_DEV int kv4_seq_of(const Kv4Rows& c, int row) {
-  const int lane = threadIdx.x & 31;
-  int n = 0;
-  for (int s = 0; s < c.n_seq; s += 32) {
-    const bool past = s + lane < c.n_seq && __ldg(c.row_start + s + lane + 1) <= row;
-    n += __popc(__ballot_sync(0xffffffffu, past));
-  }
-  return n;
-}
 
 // Cached positions of sequence s, held to its block table (an overrun is
 // reported once per call of this).
@@ -93,15 +63,22 @@ FOX_DEV int kv4_page(const Kv4Rows& c, int s, int p) {
   return -1;
 }
 
-// The row's page and position in it; false for rows that have none.
-FOX_DEV bool kv4_place(const Kv4Rows& c, int row, int* page, int* at) {
-  const int s = kv4_seq_of(c, row);
-  if (s >= c.n_seq) return false;
-  const int pos = kv4_len(c, s) - (__ldg(c.row_start + s + 1) - row);
-  if (pos < 0) return false;
-  *page = kv4_page(c, s, pos);
-  *at = pos % KV_PAGE;
-  return *page >= 0;
+// A row's page and position in it; page -1 for rows that have none.
+struct Kv4Place { int page, at; };
+FOX_DEV Kv4Place kv4_place(const Kv4Rows& c, int row) {
+  Kv4Place x = {-1, 0};
+  if (row >= c.n_rows || row < __ldg(c.row_start)) return x;
+  int lo = 0, hi = c.n_seq;  // sequences that end at or before the row
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (__ldg(c.row_start + mid + 1) <= row) lo = mid + 1; else hi = mid;
+  }
+  if (lo >= c.n_seq) return x;
+  const int pos = kv4_len(c, lo) - (__ldg(c.row_start + lo + 1) - row);
+  if (pos < 0) return x;
+  x.page = kv4_page(c, lo, pos);
+  x.at = pos % KV_PAGE;
+  return x;
 }
 
 FOX_DEV uint8_t* kv4_block(const Kv4Rows& c, int page, int head, int side, int block_bytes) {
@@ -122,122 +99,240 @@ FOX_DEV void kv4_store4(__half* p, float4 v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
+// fmaxf and fminf that a NaN goes through.
+FOX_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+FOX_DEV float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr float KV4_F16_MAX = 65504.0f;
+
 // The code of x: the k that is nearest to (x - m) / d, ties to even. x - m is
 // rounded to s (its error e exact, by Knuth's two-sum), but a code near s / d
 // leaves r = s - k d without rounding (both lie within d of each other), so
 // |r| against d / 2 decides, and e where they are equal.
-FOX_DEV uint32_t kv4_code(float x, float m, float d, float inv) {
+FOX_DEV float kv4_code(float x, float m, float d, float inv) {
+  x = fminf(fmaxf(x, -KV4_F16_MAX), KV4_F16_MAX);
   const float s = __fsub_rn(x, m);
   float k = rintf(s * inv);
   const float r = __fmaf_rn(-k, d, s), half = 0.5f * d;
-  if (fabsf(r) >= half) {
-    if (fabsf(r) > half) {
-      k += r > 0.0f ? 1.0f : -1.0f;
-    } else {
-      const float b = __fsub_rn(x, s), e = __fadd_rn(__fsub_rn(x, __fadd_rn(s, b)), __fsub_rn(b, m));
-      const float off = r > 0.0f ? e : -e;  // beyond the border (> 0), short of it, or on it
-      if (off > 0.0f || (off == 0.0f && ((int)k & 1))) k += r > 0.0f ? 1.0f : -1.0f;
-    }
+  if (fabsf(r) > half) {
+    k += r > 0.0f ? 1.0f : -1.0f;
+  } else if (fabsf(r) == half) {
+    const float b = __fsub_rn(x, s), e = __fadd_rn(__fsub_rn(x, __fadd_rn(s, b)), __fsub_rn(b, m));
+    const float off = r > 0.0f ? e : -e;  // beyond the border (> 0), short of it, or on it
+    if (off > 0.0f || (off == 0.0f && ((int)k & 1))) k += r > 0.0f ? 1.0f : -1.0f;
   }
-  return (uint32_t)(int)fminf(fmaxf(k, 0.0f), 15.0f);
+  return fminf(fmaxf(k, 0.0f), 15.0f);
 }
 
-// The group's parameters from its least and largest value. Directed
-// roundings nest: rounding up to fp32 and then to fp16 is rounding up to fp16.
-FOX_DEV __half2 kv4_pair(float lo, float hi, bool nan) {
-  if (nan) return __half2half2(__ushort_as_half(0x7fff));
-  const __half m = __float2half_rd(lo);
-  const __half d = __float2half_ru(__fdiv_ru(__fsub_ru(hi, __half2float(m)), 15.0f));
-  return __halves2half2(d, m);
-}
-
-// A group's 64 values over 16 lanes (4 each): its parameters, and this lane's
-// 4 codes as 16 bits.
-FOX_DEV uint32_t kv4_quantise(float4 x, __half2* pair) {
-  constexpr float kMax = 65504.0f;
-  bool nan = x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w;
-  x = make_float4(fminf(fmaxf(x.x, -kMax), kMax), fminf(fmaxf(x.y, -kMax), kMax), fminf(fmaxf(x.z, -kMax), kMax),
-                  fminf(fmaxf(x.w, -kMax), kMax));
-  float lo = fminf(fminf(x.x, x.y), fminf(x.z, x.w)), hi = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+// A group's 64 values over 8 lanes (8 each): its parameters, and this lane's 8
+// codes (code i in bits 4i). All parameters are exact:
+// - m: rounding down to fp16 is one instruction.
+// - d: rounding up nests (to fp32, then to fp16), and a product with 1/15
+//   rounded up is at most one fp16 too high, which 15 d' >= span tells.
+// - The codes by a product with 1 / d are, too, unless some |r| (kv4_code)
+//   reaches d / 2, where the careful form decides.
+FOX_DEV uint32_t kv4_quantise(const float (&x)[8], __half2* pair) {
+  float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  for (int i = 1; i < 8; ++i) { lo = min_nan(lo, x[i]); hi = max_nan(hi, x[i]); }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const uint32_t any = __ballot_sync(0xffffffffu, nan);
-  nan = (any >> (threadIdx.x & 16)) & 0xffffu;
-  *pair = kv4_pair(lo, hi, nan);
-  const float d = __low2float(*pair), m = __high2float(*pair);
-  if (!(d > 0.0f)) return 0;  // one value (or a NaN): every code is 0
-  const float inv = __fdiv_rn(1.0f, d);
-  return kv4_code(x.x, m, d, inv) | kv4_code(x.y, m, d, inv) << 4 | kv4_code(x.z, m, d, inv) << 8 |
-         kv4_code(x.w, m, d, inv) << 12;
+  if (lo != lo) {
+    *pair = __half2half2(__ushort_as_half(0x7fff));
+    return 0;
+  }
+  const bool wide = lo < -KV4_F16_MAX || hi > KV4_F16_MAX;
+  lo = fminf(fmaxf(lo, -KV4_F16_MAX), KV4_F16_MAX);
+  hi = fminf(fmaxf(hi, -KV4_F16_MAX), KV4_F16_MAX);
+  const __half m16 = __float2half_rd(lo);
+  const float m = __half2float(m16), span = __fsub_ru(hi, m);
+  __half d16 = __float2half_ru(__fmul_ru(span, 0x1.111112p-4f));
+  const __half less = __ushort_as_half((unsigned short)(__half_as_ushort(d16) - 1));
+  if (span > 0.0f && 15.0f * __half2float(less) >= span) d16 = less;
+  const float d = __half2float(d16);
+  *pair = __halves2half2(d16, m16);
+  if (d == 0.0f) return 0;  // one value: every code is 0
+  const float inv = __fdividef(1.0f, d), magic = 12582912.0f;  // adding 1.5 * 2^23 rounds to a whole number
+  float k[8], far = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float s = __fsub_rn(x[i], m);
+    k[i] = __fsub_rn(__fmaf_rn(s, inv, magic), magic);
+    far = fmaxf(far, fabsf(__fmaf_rn(-k[i], d, s)));
+  }
+  if (wide || far >= 0.5f * d) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = kv4_code(x[i], m, d, inv);
+  }
+  const float a = __fmaf_rn(__fmaf_rn(__fmaf_rn(k[3], 16.0f, k[2]), 16.0f, k[1]), 16.0f, k[0]);
+  const float b = __fmaf_rn(__fmaf_rn(__fmaf_rn(k[7], 16.0f, k[6]), 16.0f, k[5]), 16.0f, k[4]);
+  return (uint32_t)a | (uint32_t)b << 16;
 }
 
-struct Kv4WriteParams {
+// Byte offsets in a block: of the word that holds dimensions d .. d+7 of
+// position `at` (K), of the half word of d .. d+3 (V), of a group's parameters.
+template <int HD>
+struct Kv4Lay {
+  static constexpr int SLAB = HD < 128 ? HD : 128, SG = SLAB / 64, NB = SLAB / 32, G = HD / KV4_GROUP;
+  static FOX_DEV int k(int at, int d) {
+    const int r = d % SLAB;
+    return d / SLAB * (KV_PAGE * SLAB / 2) + at * (SLAB / 2) + r % 64 / 16 * 8 * SG + 8 * (r / 64) + 4 * (r % 16 / 8);
+  }
+  static FOX_DEV int v(int at, int d) {
+    const int r = d % SLAB;
+    return ((((d / SLAB * 4 + at / 16) * 2 + at / 8 % 2) * 4 + at % 8 / 2) * 8 + r % 32 / 4) * 4 * NB + 4 * (r / 32) + 2 * (at & 1);
+  }
+  static FOX_DEV int pair(int at, int group) { return kv4_codes_bytes(HD) + 4 * (at * G + group); }
+};
+
+// 8 values from and to 16-byte aligned memory.
+FOX_DEV void kv4_load8(const float* p, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+FOX_DEV void kv4_load8(const __half* p, float (&v)[8]) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x; v[2 * i + 1] = f.y;
+  }
+}
+FOX_DEV void kv4_store8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+FOX_DEV void kv4_store8(__half* p, const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct Kv4MoveParams {
   Kv4Rows c;
-  const void *k, *v;
+  void *k, *v;                // rows to write into the cache, or read back from it
   size_t k_stride, v_stride;  // elements between rows
 };
 
-// One warp quantises a row's K and V of one head: 16 lanes a group.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4WriteParams p) {
+// What a warp moves of a row at a time: four groups, 8 lanes each, a lane 8
+// dimensions. They are K and V of two heads (64 dimensions), of one head
+// (128), or K or V of one head (256). Pass q of a row begins at head first(q);
+// a lane's offsets in a block and in a head are the same in every pass.
+template <int HD>
+struct Kv4Pass {
+  using Y = Kv4Lay<HD>;
+  static constexpr int G = Y::G;
+  int sub, g, d;
+  FOX_DEV Kv4Pass() : sub((threadIdx.x & 31) >> 3), g(sub % G), d(sub % G * KV4_GROUP + 8 * (threadIdx.x & 7)) {}
+  static __host__ __device__ constexpr int passes(int n_kv) { return G == 1 ? (n_kv + 1) / 2 : G == 2 ? n_kv : 2 * n_kv; }
+  FOX_DEV int head(int q) const { return G == 1 ? 2 * q + (sub >> 1) : G == 2 ? q : q >> 1; }
+  FOX_DEV int side(int q) const { return G == 1 ? sub & 1 : G == 2 ? sub >> 1 : q & 1; }
+};
+
+// A warp takes BATCH passes of a row.
+template <typename T, int HD, int BATCH>
+__global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4MoveParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  constexpr int G = HD / KV4_GROUP, BB = kv4_block_bytes(HD);
-  const int lane = threadIdx.x & 31;
-  const size_t unit = blockIdx.x * (size_t)(blockDim.x / 32) + threadIdx.x / 32;
-  if (unit >= (size_t)p.c.n_rows * p.c.n_kv) return;
-  const int row = (int)(unit / p.c.n_kv), head = (int)(unit - (size_t)row * p.c.n_kv);
-  int page, at;
-  if (!kv4_place(p.c, row, &page, &at)) return;
-  const T* src[2] = {static_cast<const T*>(p.k) + row * p.k_stride + head * HD,
-                     static_cast<const T*>(p.v) + row * p.v_stride + head * HD};
-  uint8_t* block = kv4_block(p.c, page, head, 0, BB);
-  // 2 G groups of 64 dimensions: K's, then V's; each half warp takes one
+  using Y = Kv4Lay<HD>;
+  constexpr int BB = kv4_block_bytes(HD);
+  const Kv4Pass<HD> pass;
+  const int passes = pass.passes(p.c.n_kv), chunks = (passes + BATCH - 1) / BATCH;
+  const unsigned unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;  // below 2^20 rows * 2^11 chunks
+  const int row = (int)(unit / chunks), q0 = (int)(unit - row * chunks) * BATCH;
+  if (row >= p.c.n_rows) return;
+  const T* src[2] = {static_cast<const T*>(p.k) + row * p.k_stride + pass.d, static_cast<const T*>(p.v) + row * p.v_stride + pass.d};
+  float x[BATCH][8];
 #pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const int u = 2 * i + (lane >> 4), side = u / G, g = u % G, d = g * KV4_GROUP + 4 * (lane & 15);
+  for (int b = 0; b < BATCH; ++b)  // on their way while the row's place is found
+    kv4_load8(src[pass.side(q0 + b)] + min(pass.head(q0 + b), p.c.n_kv - 1) * HD, x[b]);
+  const Kv4Place at = kv4_place(p.c, row);
+  if (at.page < 0) return;
+  uint8_t* page = kv4_block(p.c, at.page, 0, 0, BB);
+  const int k_at = Y::k(at.at, pass.d), v_at = BB + Y::v(at.at, pass.d), v_at4 = BB + Y::v(at.at, pass.d + 4);
+  const int pair_at = Y::pair(at.at, pass.g);
+#pragma unroll
+  for (int b = 0; b < BATCH; ++b) {
+    const int head = pass.head(q0 + b);
     __half2 pair;
-    const uint32_t code = kv4_quantise(kv4_load4(src[side] + d), &pair);
-    uint8_t* b = block + side * BB;
-    *reinterpret_cast<uint16_t*>(b + (side ? kv4_v_at<HD>(at, d) : kv4_k_at<HD>(at, d))) = (uint16_t)code;
-    if ((lane & 15) == 0) *reinterpret_cast<__half2*>(b + kv4_codes_bytes(HD) + 4 * (at * G + g)) = pair;
+    const uint32_t code = kv4_quantise(x[b], &pair);
+    if (head >= p.c.n_kv) continue;
+    uint8_t* block = page + head * (2 * BB);
+    if (pass.side(q0 + b)) {
+      *reinterpret_cast<uint16_t*>(block + v_at) = (uint16_t)code;
+      *reinterpret_cast<uint16_t*>(block + v_at4) = (uint16_t)(code >> 16);
+    } else {
+      *reinterpret_cast<uint32_t*>(block + k_at) = code;
+    }
+    if ((threadIdx.x & 7) == 0) *reinterpret_cast<__half2*>(block + pass.side(q0 + b) * BB + pair_at) = pair;
   }
 }
 
-struct Kv4ReadParams {
-  Kv4Rows c;
-  void *k, *v;
-};
-
-FOX_DEV float4 kv4_decode(uint32_t code, __half2 pair) {
-  const float d = __low2float(pair), m = __high2float(pair);
-  return make_float4(__fmaf_rn(d, (float)(code & 15), m), __fmaf_rn(d, (float)(code >> 4 & 15), m),
-                     __fmaf_rn(d, (float)(code >> 8 & 15), m), __fmaf_rn(d, (float)(code >> 12 & 15), m));
+// 8 codes (code i in bits 4i) as the values they stand for. A code in a half's
+// mantissa is a subnormal, c * 2^-22 in bits 2-5 and c * 2^-18 in bits 6-9; d
+// takes the power of two back, exactly.
+FOX_DEV void kv4_decode(uint32_t code, __half2 pair, float (&v)[8]) {
+  const float m = __high2float(pair), d0 = __low2float(pair) * 4194304.0f, d1 = d0 * 0.0625f;
+  const uint32_t up = code << 2, down = code >> 6;
+  const uint32_t w[4] = {up & 0x003c003cu, up & 0x03c003c0u, down & 0x003c003cu, down & 0x03c003c0u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[i] = __fmaf_rn(i % 2 ? d1 : d0, f.x, m);
+    v[i + 4] = __fmaf_rn(i % 2 ? d1 : d0, f.y, m);
+  }
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
+template <typename T, int HD, int BATCH>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4MoveParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  constexpr int G = HD / KV4_GROUP, BB = kv4_block_bytes(HD);
-  const int lane = threadIdx.x & 31;
-  const size_t unit = blockIdx.x * (size_t)(blockDim.x / 32) + threadIdx.x / 32;
-  if (unit >= (size_t)p.c.n_rows * p.c.n_kv) return;
-  const int row = (int)(unit / p.c.n_kv), head = (int)(unit - (size_t)row * p.c.n_kv);
-  int page, at;
-  if (!kv4_place(p.c, row, &page, &at)) return;
-  const uint8_t* block = kv4_block(p.c, page, head, 0, BB);
+  using Y = Kv4Lay<HD>;
+  constexpr int BB = kv4_block_bytes(HD);
+  const Kv4Pass<HD> pass;
+  const int passes = pass.passes(p.c.n_kv), chunks = (passes + BATCH - 1) / BATCH;
+  const unsigned unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const int row = (int)(unit / chunks), q0 = (int)(unit - row * chunks) * BATCH;
+  if (row >= p.c.n_rows) return;
+  const Kv4Place at = kv4_place(p.c, row);
+  if (at.page < 0) return;
+  const uint8_t* page = kv4_block(p.c, at.page, 0, 0, BB);
+  const int k_at = Y::k(at.at, pass.d), v_at = BB + Y::v(at.at, pass.d), v_at4 = BB + Y::v(at.at, pass.d + 4);
+  const int pair_at = Y::pair(at.at, pass.g);
+  uint32_t code[BATCH];
+  __half2 pair[BATCH];
 #pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const int u = 2 * i + (lane >> 4), side = u / G, g = u % G, d = g * KV4_GROUP + 4 * (lane & 15);
-    const uint8_t* b = block + side * BB;
-    const uint32_t code = *reinterpret_cast<const uint16_t*>(b + (side ? kv4_v_at<HD>(at, d) : kv4_k_at<HD>(at, d)));
-    const __half2 pair = *reinterpret_cast<const __half2*>(b + kv4_codes_bytes(HD) + 4 * (at * G + g));
-    T* out = static_cast<T*>(side ? p.v : p.k) + unit * HD + d;
-    kv4_store4(out, kv4_decode(code, pair));
+  for (int b = 0; b < BATCH; ++b) {
+    const uint8_t* block = page + min(pass.head(q0 + b), p.c.n_kv - 1) * (2 * BB);
+    code[b] = pass.side(q0 + b) ? *reinterpret_cast<const uint16_t*>(block + v_at) |
+                                      (uint32_t) * reinterpret_cast<const uint16_t*>(block + v_at4) << 16
+                                : *reinterpret_cast<const uint32_t*>(block + k_at);
+    pair[b] = *reinterpret_cast<const __half2*>(block + pass.side(q0 + b) * BB + pair_at);
+  }
+  T* dst[2] = {static_cast<T*>(p.k) + (size_t)row * p.c.n_kv * HD + pass.d, static_cast<T*>(p.v) + (size_t)row * p.c.n_kv * HD + pass.d};
+#pragma unroll
+  for (int b = 0; b < BATCH; ++b) {
+    const int head = pass.head(q0 + b);
+    if (head >= p.c.n_kv) break;
+    float v[8];
+    kv4_decode(code[b], pair[b], v);
+    kv4_store8(dst[pass.side(q0 + b)] + head * HD, v);
   }
 }
 
@@ -253,66 +348,105 @@ struct RopeParams {
   int* err;
 };
 
+FOX_DEV void rope_load(const float* p, float (&v)[8]) { kv4_load8(p, v); }
+FOX_DEV void rope_load(const __half* p, float (&v)[8]) { kv4_load8(p, v); }
+FOX_DEV void rope_load(const float* p, float (&v)[4]) {
+  const float4 x = *reinterpret_cast<const float4*>(p);
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+FOX_DEV void rope_store(float* p, const float (&v)[8]) { kv4_store8(p, v); }
+FOX_DEV void rope_store(__half* p, const float (&v)[8]) { kv4_store8(p, v); }
+FOX_DEV void rope_store(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
 // RMSNorm of every query and key head and the rotation of its position:
 //   y = x * (1 / sqrt(mean(x^2) + eps)) * w
 //   (a, b) -> (a cos - b sin, a sin + b cos) for the pairs (2i, 2i+1), or
 //   (i, i + hd/2) when halves is set.
-// One warp a head: a lane holds HD/32 neighbouring dimensions, so the pairs
-// lie in a lane and the halves 16 lanes apart. Without norms the result is
-// that of the decode step's rotation, bit for bit.
+// A lane holds E neighbouring dimensions of a head (16 bytes, or 32 of 256
+// fp32 dimensions), so the pairs lie in a lane and the halves LANES / 2 lanes
+// apart. A warp takes BATCH such loads of one row's query or key heads, so that
+// the row's sines, cosines and the weights are loaded once for all of them and
+// the loads are in flight together. Without norms the result is that of the
+// decode step's rotation, bit for bit.
 template <typename T, int HD>
+struct RopeLay {
+  static constexpr int E = sizeof(T) == 2 || HD == 256 ? 8 : 4, LANES = HD / E, AT_ONCE = 32 / LANES;
+  static __host__ __device__ int chunks(int heads, int batch) { return (heads + AT_ONCE * batch - 1) / (AT_ONCE * batch); }
+};
+template <typename T, int HD, bool HALVES, int BATCH>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const RopeParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  constexpr int E = HD / 32;
-  const int lane = threadIdx.x & 31, heads = p.n_head + p.n_kv;
-  const size_t unit = blockIdx.x * (size_t)(blockDim.x / 32) + threadIdx.x / 32;
-  if (unit >= (size_t)p.n_rows * heads) return;
-  const int row = (int)(unit / heads), h = (int)(unit - (size_t)row * heads);
+  using Y = RopeLay<T, HD>;
+  constexpr int E = Y::E, LANES = Y::LANES, AT_ONCE = Y::AT_ONCE, C = HALVES ? E : E / 2;
+  const int lane = threadIdx.x & 31, sub = lane / LANES, l = lane % LANES;
+  const int q_chunks = Y::chunks(p.n_head, BATCH), chunks = q_chunks + Y::chunks(p.n_kv, BATCH);
+  const unsigned unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;  // below 2^20 rows * 2^11 chunks
+  const int row = (int)(unit / chunks), chunk = (int)(unit - row * chunks);
+  if (row >= p.n_rows) return;
+  const bool is_q = chunk < q_chunks;
+  const int heads = is_q ? p.n_head : p.n_kv, h0 = (is_q ? chunk : chunk - q_chunks) * (AT_ONCE * BATCH) + sub;
   const int pos = __ldg(p.pos + row);
   if (pos < 0) return;
+  const T* x = static_cast<const T*>(p.x) + (size_t)row * p.x_stride + (size_t)(is_q ? 0 : p.n_head) * HD + l * E;
+  float v[BATCH][E];
+#pragma unroll
+  for (int b = 0; b < BATCH; ++b) rope_load(x + (size_t)min(h0 + b * AT_ONCE, heads - 1) * HD, v[b]);
   if (pos >= p.n_pos) {
     if (lane == 0 && p.err) atomicExch(p.err, KERR_PAGES);
     return;
   }
-  const bool is_q = h < p.n_head;
-  const T* x = static_cast<const T*>(p.x) + row * p.x_stride + (size_t)h * HD + lane * E;
-  float v[E];
+  float cs[C], sn[C];
+  {
+    const int i0 = HALVES ? l % (LANES / 2) * E : l * (E / 2);
+    const float *c = p.cos + (size_t)pos * (HD / 2) + i0, *s = p.sin + (size_t)pos * (HD / 2) + i0;
 #pragma unroll
-  for (int i = 0; i < E; ++i) v[i] = (float)x[i];
-  const float* w = is_q ? p.q_norm : p.k_norm;
-  if (w) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
-    const float scale = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(warp_sum(ss), (float)HD), p.eps)));
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], scale), __ldg(w + lane * E + i));
-  }
-  const float* cs = p.cos + (size_t)pos * (HD / 2);
-  const float* sn = p.sin + (size_t)pos * (HD / 2);
-  float o[E];
-  if (p.halves) {
-    const int i0 = (lane & 15) * E;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float other = __shfl_xor_sync(0xffffffffu, v[i], 16);
-      const float c = __ldg(cs + i0 + i), s = __ldg(sn + i0 + i);
-      o[i] = lane < 16 ? __fsub_rn(__fmul_rn(v[i], c), __fmul_rn(other, s))
-                       : __fadd_rn(__fmul_rn(other, s), __fmul_rn(v[i], c));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const float c = __ldg(cs + (lane * E + i) / 2), s = __ldg(sn + (lane * E + i) / 2);
-      o[i] = __fsub_rn(__fmul_rn(v[i], c), __fmul_rn(v[i + 1], s));
-      o[i + 1] = __fadd_rn(__fmul_rn(v[i], s), __fmul_rn(v[i + 1], c));
+    for (int i = 0; i < C; i += 2) {
+      const float2 a = __ldg(reinterpret_cast<const float2*>(c + i)), b = __ldg(reinterpret_cast<const float2*>(s + i));
+      cs[i] = a.x; cs[i + 1] = a.y; sn[i] = b.x; sn[i + 1] = b.y;
     }
   }
-  T* out = is_q ? static_cast<T*>(p.q) + row * p.q_stride + (size_t)h * HD
-                : static_cast<T*>(p.k) + row * p.k_stride + (size_t)(h - p.n_head) * HD;
+  const float* norm = is_q ? p.q_norm : p.k_norm;
+  float w[E];
+  if (norm) rope_load(norm + l * E, w);
+  T* out = is_q ? static_cast<T*>(p.q) + (size_t)row * p.q_stride : static_cast<T*>(p.k) + (size_t)row * p.k_stride;
+  out += l * E;
 #pragma unroll
-  for (int i = 0; i < E; ++i) out[lane * E + i] = (T)o[i];
+  for (int b = 0; b < BATCH; ++b) {
+    const int h = h0 + b * AT_ONCE;
+    if (norm) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) ss = fmaf(v[b][i], v[b][i], ss);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float mean = fmaf(ss, 1.0f / HD, p.eps);
+      float scale = rsqrtf(mean);
+      scale = fmaf(0.5f * scale, fmaf(-mean * scale, scale, 1.0f), scale);  // a Newton step: the last bits
+      // (an infinite mean, or zero with no eps, has nothing to refine)
+      if (!(mean > 0.0f) || isinf(mean)) scale = rsqrtf(mean);
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[b][i] = __fmul_rn(__fmul_rn(v[b][i], scale), w[i]);
+    }
+    float o[E];
+    if (HALVES) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, v[b][i], LANES / 2);
+        o[i] = l < LANES / 2 ? __fsub_rn(__fmul_rn(v[b][i], cs[i]), __fmul_rn(other, sn[i]))
+                             : __fadd_rn(__fmul_rn(other, sn[i]), __fmul_rn(v[b][i], cs[i]));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        o[i] = __fsub_rn(__fmul_rn(v[b][i], cs[i / 2]), __fmul_rn(v[b][i + 1], sn[i / 2]));
+        o[i + 1] = __fadd_rn(__fmul_rn(v[b][i], sn[i / 2]), __fmul_rn(v[b][i + 1], cs[i / 2]));
+      }
+    }
+    if (h < heads) rope_store(out + (size_t)h * HD, o);
+  }
 }
 
 }  // namespace fox
