@@ -63,12 +63,12 @@ static cudaError_t by_type_hd(int type, uint32_t hd, F f) {
   return type == T_F32 ? with(float()) : with(__half());
 }
 
-// One pass a warp where the rows are few, so that they spread over the device;
-// four, for one search for the row's place, where they fill it anyway.
+// One row a warp where the rows are few, so that they spread over the device;
+// four, for one search for their places, where they fill it anyway.
 template <int HD, typename F>
-static cudaError_t by_batch(const Kv4Rows& c, F f) {
+static cudaError_t by_rows(const Kv4Rows& c, F f) {
   const int passes = Kv4Pass<HD>::passes(c.n_kv);
-  const auto grid = [&](int batch) { return (unsigned)(((size_t)c.n_rows * ((passes + batch - 1) / batch) + 7) / 8); };
+  const auto grid = [&](int rows) { return (unsigned)(((size_t)((c.n_rows + rows - 1) / rows) * passes + 7) / 8); };
   if ((long long)c.n_rows * passes > 32LL * current_sms()) f(std::integral_constant<int, 4>(), grid(4));
   else f(std::integral_constant<int, 1>(), grid(1));
   return cudaGetLastError();
@@ -86,8 +86,8 @@ extern "C" foxcuda_status foxcuda_kv4_write(const foxcuda_kv4* c, int type, cons
     return fail(FOXCUDA_ERR_ARG, "kv4_write: rows must be 16-byte aligned and at least a row apart");
   p.k = const_cast<void*>(k); p.v = const_cast<void*>(v); p.k_stride = k_stride; p.v_stride = v_stride;
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
-       return by_batch<hd.value>(p.c, [&](auto batch, unsigned grid) {
-         kv4_write_kernel<decltype(tag), hd.value, batch.value><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+       return by_rows<hd.value>(p.c, [&](auto rows, unsigned grid) {
+         kv4_write_kernel<decltype(tag), hd.value, rows.value><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
        });
      }), "kv4_write launch");
   return FOXCUDA_OK;
@@ -102,8 +102,8 @@ extern "C" foxcuda_status foxcuda_kv4_read(const foxcuda_kv4* c, int type, void*
   if (!aligned16(k) || !aligned16(v)) return fail(FOXCUDA_ERR_ARG, "kv4_read: rows must be 16-byte aligned");
   p.k = k; p.v = v;
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
-       return by_batch<hd.value>(p.c, [&](auto batch, unsigned grid) {
-         kv4_read_kernel<decltype(tag), hd.value, batch.value><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+       return by_rows<hd.value>(p.c, [&](auto rows, unsigned grid) {
+         kv4_read_kernel<decltype(tag), hd.value, rows.value><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
        });
      }), "kv4_read launch");
   return FOXCUDA_OK;

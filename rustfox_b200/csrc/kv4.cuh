@@ -181,19 +181,22 @@ FOX_DEV uint32_t kv4_quantise(const float (&x)[8], __half2* pair) {
 }
 
 // Byte offsets in a block: of the word that holds dimensions d .. d+7 of
-// position `at` (K), of the half word of d .. d+3 (V), of a group's parameters.
+// position `at` (K), of the half word of d .. d+3 (V), of a group's
+// parameters; each is a sum of a part of the position and one of the dimension.
 template <int HD>
 struct Kv4Lay {
   static constexpr int SLAB = HD < 128 ? HD : 128, SG = SLAB / 64, NB = SLAB / 32, G = HD / KV4_GROUP;
-  static FOX_DEV int k(int at, int d) {
+  static FOX_DEV int k_row(int at) { return at * (SLAB / 2); }
+  static FOX_DEV int k_dim(int d) {
     const int r = d % SLAB;
-    return d / SLAB * (KV_PAGE * SLAB / 2) + at * (SLAB / 2) + r % 64 / 16 * 8 * SG + 8 * (r / 64) + 4 * (r % 16 / 8);
+    return d / SLAB * (KV_PAGE * SLAB / 2) + r % 64 / 16 * 8 * SG + 8 * (r / 64) + 4 * (r % 16 / 8);
   }
-  static FOX_DEV int v(int at, int d) {
+  static FOX_DEV int v_row(int at) { return at / 2 * (8 * 4 * NB) + 2 * (at & 1); }
+  static FOX_DEV int v_dim(int d) {
     const int r = d % SLAB;
-    return ((((d / SLAB * 4 + at / 16) * 2 + at / 8 % 2) * 4 + at % 8 / 2) * 8 + r % 32 / 4) * 4 * NB + 4 * (r / 32) + 2 * (at & 1);
+    return d / SLAB * (KV_PAGE * SLAB / 2) + r % 32 / 4 * 4 * NB + 4 * (r / 32);
   }
-  static FOX_DEV int pair(int at, int group) { return kv4_codes_bytes(HD) + 4 * (at * G + group); }
+  static FOX_DEV int pair_row(int at) { return kv4_codes_bytes(HD) + at * (4 * G); }
 };
 
 // 8 values from and to 16-byte aligned memory.
@@ -230,57 +233,79 @@ struct Kv4MoveParams {
   size_t k_stride, v_stride;  // elements between rows
 };
 
-// What a warp moves of a row at a time: four groups, 8 lanes each, a lane 8
-// dimensions. They are K and V of two heads (64 dimensions), of one head
-// (128), or K or V of one head (256). Pass q of a row begins at head first(q);
-// a lane's offsets in a block and in a head are the same in every pass.
+// What a warp moves of each of its rows: pass q of the row, four groups, 8
+// lanes each, a lane 8 dimensions. The groups are K and V of two heads (64
+// dimensions), of one head (128), or K or V of one head (256).
 template <int HD>
 struct Kv4Pass {
-  using Y = Kv4Lay<HD>;
-  static constexpr int G = Y::G;
-  int sub, g, d;
-  FOX_DEV Kv4Pass() : sub((threadIdx.x & 31) >> 3), g(sub % G), d(sub % G * KV4_GROUP + 8 * (threadIdx.x & 7)) {}
+  static constexpr int G = HD / KV4_GROUP;
+  int head, side, d;
+  bool live;       // the second head of an odd number's last pass is not
+  size_t in_page;  // byte of the lane's block in a page
+  int code_dim, code_dim4, pair_dim;
+  FOX_DEV Kv4Pass(int q, int n_kv) {
+    using Y = Kv4Lay<HD>;
+    const int sub = (threadIdx.x & 31) >> 3;
+    head = G == 1 ? 2 * q + (sub >> 1) : G == 2 ? q : q >> 1;
+    side = G == 1 ? sub & 1 : G == 2 ? sub >> 1 : q & 1;
+    live = head < n_kv;
+    head = min(head, n_kv - 1);
+    d = sub % G * KV4_GROUP + 8 * (threadIdx.x & 7);
+    in_page = (size_t)(2 * head + side) * kv4_block_bytes(HD);
+    code_dim = side ? Y::v_dim(d) : Y::k_dim(d);
+    code_dim4 = Y::v_dim(d + 4);
+    pair_dim = 4 * (sub % G);
+  }
   static __host__ __device__ constexpr int passes(int n_kv) { return G == 1 ? (n_kv + 1) / 2 : G == 2 ? n_kv : 2 * n_kv; }
-  FOX_DEV int head(int q) const { return G == 1 ? 2 * q + (sub >> 1) : G == 2 ? q : q >> 1; }
-  FOX_DEV int side(int q) const { return G == 1 ? sub & 1 : G == 2 ? sub >> 1 : q & 1; }
 };
+// A warp's rows: ROWS neighbouring ones, their places found by as many lanes
+// at once. Unit u is pass u % passes of rows u / passes * ROWS on.
+template <int ROWS>
+FOX_DEV Kv4Place kv4_places(const Kv4Rows& c, int row0) {
+  const int lane = threadIdx.x & 31;
+  Kv4Place x = {-1, 0};
+  if (lane < ROWS) x = kv4_place(c, row0 + lane);
+  return x;
+}
 
-// A warp takes BATCH passes of a row.
-template <typename T, int HD, int BATCH>
+constexpr int KV4_AT_ONCE = 4;  // rows whose loads are in flight together
+
+template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4MoveParams p) {
   griddep_wait();
   griddep_launch_dependents();
   using Y = Kv4Lay<HD>;
-  constexpr int BB = kv4_block_bytes(HD);
-  const Kv4Pass<HD> pass;
-  const int passes = pass.passes(p.c.n_kv), chunks = (passes + BATCH - 1) / BATCH;
-  const unsigned unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;  // below 2^20 rows * 2^11 chunks
-  const int row = (int)(unit / chunks), q0 = (int)(unit - row * chunks) * BATCH;
-  if (row >= p.c.n_rows) return;
-  const T* src[2] = {static_cast<const T*>(p.k) + row * p.k_stride + pass.d, static_cast<const T*>(p.v) + row * p.v_stride + pass.d};
-  float x[BATCH][8];
+  constexpr int N = ROWS < KV4_AT_ONCE ? ROWS : KV4_AT_ONCE;
+  const unsigned unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, passes = Kv4Pass<HD>::passes(p.c.n_kv);
+  const int row0 = (int)(unit / passes) * ROWS;
+  if (row0 >= p.c.n_rows) return;
+  const Kv4Pass<HD> pass((int)(unit % passes), p.c.n_kv);
+  const T* src = static_cast<const T*>(pass.side ? p.v : p.k) + pass.head * HD + pass.d;
+  const size_t stride = pass.side ? p.v_stride : p.k_stride, page_bytes = (size_t)p.c.n_kv * 2 * kv4_block_bytes(HD);
+  Kv4Place mine;
 #pragma unroll
-  for (int b = 0; b < BATCH; ++b)  // on their way while the row's place is found
-    kv4_load8(src[pass.side(q0 + b)] + min(pass.head(q0 + b), p.c.n_kv - 1) * HD, x[b]);
-  const Kv4Place at = kv4_place(p.c, row);
-  if (at.page < 0) return;
-  uint8_t* page = kv4_block(p.c, at.page, 0, 0, BB);
-  const int k_at = Y::k(at.at, pass.d), v_at = BB + Y::v(at.at, pass.d), v_at4 = BB + Y::v(at.at, pass.d + 4);
-  const int pair_at = Y::pair(at.at, pass.g);
+  for (int r0 = 0; r0 < ROWS; r0 += N) {
+    float x[N][8];
 #pragma unroll
-  for (int b = 0; b < BATCH; ++b) {
-    const int head = pass.head(q0 + b);
-    __half2 pair;
-    const uint32_t code = kv4_quantise(x[b], &pair);
-    if (head >= p.c.n_kv) continue;
-    uint8_t* block = page + head * (2 * BB);
-    if (pass.side(q0 + b)) {
-      *reinterpret_cast<uint16_t*>(block + v_at) = (uint16_t)code;
-      *reinterpret_cast<uint16_t*>(block + v_at4) = (uint16_t)(code >> 16);
-    } else {
-      *reinterpret_cast<uint32_t*>(block + k_at) = code;
+    for (int i = 0; i < N; ++i) kv4_load8(src + min(row0 + r0 + i, p.c.n_rows - 1) * stride, x[i]);
+    if (r0 == 0) mine = kv4_places<ROWS>(p.c, row0);  // while the first rows are on their way
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int page = __shfl_sync(0xffffffffu, mine.page, r0 + i), at = __shfl_sync(0xffffffffu, mine.at, r0 + i);
+      if (page < 0) continue;
+      __half2 pair;
+      const uint32_t code = kv4_quantise(x[i], &pair);
+      if (!pass.live) continue;
+      uint8_t* block = p.c.cache + page * page_bytes + pass.in_page;
+      if (pass.side) {
+        uint8_t* dst = block + Y::v_row(at);
+        *reinterpret_cast<uint16_t*>(dst + pass.code_dim) = (uint16_t)code;
+        *reinterpret_cast<uint16_t*>(dst + pass.code_dim4) = (uint16_t)(code >> 16);
+      } else {
+        *reinterpret_cast<uint32_t*>(block + Y::k_row(at) + pass.code_dim) = code;
+      }
+      if ((threadIdx.x & 7) == 0) *reinterpret_cast<__half2*>(block + Y::pair_row(at) + pass.pair_dim) = pair;
     }
-    if ((threadIdx.x & 7) == 0) *reinterpret_cast<__half2*>(block + pass.side(q0 + b) * BB + pair_at) = pair;
   }
 }
 
@@ -299,40 +324,46 @@ FOX_DEV void kv4_decode(uint32_t code, __half2 pair, float (&v)[8]) {
   }
 }
 
-template <typename T, int HD, int BATCH>
+template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4MoveParams p) {
   griddep_wait();
   griddep_launch_dependents();
   using Y = Kv4Lay<HD>;
-  constexpr int BB = kv4_block_bytes(HD);
-  const Kv4Pass<HD> pass;
-  const int passes = pass.passes(p.c.n_kv), chunks = (passes + BATCH - 1) / BATCH;
-  const unsigned unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  const int row = (int)(unit / chunks), q0 = (int)(unit - row * chunks) * BATCH;
-  if (row >= p.c.n_rows) return;
-  const Kv4Place at = kv4_place(p.c, row);
-  if (at.page < 0) return;
-  const uint8_t* page = kv4_block(p.c, at.page, 0, 0, BB);
-  const int k_at = Y::k(at.at, pass.d), v_at = BB + Y::v(at.at, pass.d), v_at4 = BB + Y::v(at.at, pass.d + 4);
-  const int pair_at = Y::pair(at.at, pass.g);
-  uint32_t code[BATCH];
-  __half2 pair[BATCH];
+  constexpr int N = ROWS < KV4_AT_ONCE ? ROWS : KV4_AT_ONCE;
+  const unsigned unit = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, passes = Kv4Pass<HD>::passes(p.c.n_kv);
+  const int row0 = (int)(unit / passes) * ROWS;
+  if (row0 >= p.c.n_rows) return;
+  const Kv4Pass<HD> pass((int)(unit % passes), p.c.n_kv);
+  const Kv4Place mine = kv4_places<ROWS>(p.c, row0);
+  const size_t page_bytes = (size_t)p.c.n_kv * 2 * kv4_block_bytes(HD);
+  T* dst = static_cast<T*>(pass.side ? p.v : p.k) + ((size_t)row0 * p.c.n_kv + pass.head) * HD + pass.d;
 #pragma unroll
-  for (int b = 0; b < BATCH; ++b) {
-    const uint8_t* block = page + min(pass.head(q0 + b), p.c.n_kv - 1) * (2 * BB);
-    code[b] = pass.side(q0 + b) ? *reinterpret_cast<const uint16_t*>(block + v_at) |
-                                      (uint32_t) * reinterpret_cast<const uint16_t*>(block + v_at4) << 16
-                                : *reinterpret_cast<const uint32_t*>(block + k_at);
-    pair[b] = *reinterpret_cast<const __half2*>(block + pass.side(q0 + b) * BB + pair_at);
-  }
-  T* dst[2] = {static_cast<T*>(p.k) + (size_t)row * p.c.n_kv * HD + pass.d, static_cast<T*>(p.v) + (size_t)row * p.c.n_kv * HD + pass.d};
+  for (int r0 = 0; r0 < ROWS; r0 += N) {
+    uint32_t code[N];
+    __half2 pair[N];
+    bool there[N];
 #pragma unroll
-  for (int b = 0; b < BATCH; ++b) {
-    const int head = pass.head(q0 + b);
-    if (head >= p.c.n_kv) break;
-    float v[8];
-    kv4_decode(code[b], pair[b], v);
-    kv4_store8(dst[pass.side(q0 + b)] + head * HD, v);
+    for (int i = 0; i < N; ++i) {
+      const int page = __shfl_sync(0xffffffffu, mine.page, r0 + i), at = __shfl_sync(0xffffffffu, mine.at, r0 + i);
+      there[i] = page >= 0 && pass.live;
+      const uint8_t* block = p.c.cache + max(page, 0) * page_bytes + pass.in_page;
+      if (!there[i]) continue;
+      if (pass.side) {
+        const uint8_t* from = block + Y::v_row(at);
+        code[i] = *reinterpret_cast<const uint16_t*>(from + pass.code_dim) |
+                  (uint32_t) * reinterpret_cast<const uint16_t*>(from + pass.code_dim4) << 16;
+      } else {
+        code[i] = *reinterpret_cast<const uint32_t*>(block + Y::k_row(at) + pass.code_dim);
+      }
+      pair[i] = *reinterpret_cast<const __half2*>(block + Y::pair_row(at) + pass.pair_dim);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!there[i]) continue;
+      float v[8];
+      kv4_decode(code[i], pair[i], v);
+      kv4_store8(dst + (size_t)(r0 + i) * p.c.n_kv * HD, v);
+    }
   }
 }
 
@@ -348,17 +379,36 @@ struct RopeParams {
   int* err;
 };
 
-FOX_DEV void rope_load(const float* p, float (&v)[8]) { kv4_load8(p, v); }
-FOX_DEV void rope_load(const __half* p, float (&v)[8]) { kv4_load8(p, v); }
-FOX_DEV void rope_load(const float* p, float (&v)[4]) {
-  const float4 x = *reinterpret_cast<const float4*>(p);
-  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+// E neighbouring values as they lie in memory, and as floats.
+template <typename T, int E>
+struct RopeVec {
+  uint4 u[E * sizeof(T) / 16];
+  FOX_DEV void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  FOX_DEV void get(float (&v)[E]) const {
+#pragma unroll
+    for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) {
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          v[4 * i + j] = __uint_as_float(w[j]);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          v[2 * j] = f.x; v[2 * j + 1] = f.y;
+        }
+      }
+    }
+  }
+};
+template <int E>
+FOX_DEV void rope_store(float* p, const float (&v)[E]) {
+#pragma unroll
+  for (int i = 0; i < E; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
 }
-FOX_DEV void rope_store(float* p, const float (&v)[8]) { kv4_store8(p, v); }
 FOX_DEV void rope_store(__half* p, const float (&v)[8]) { kv4_store8(p, v); }
-FOX_DEV void rope_store(float* p, const float (&v)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-}
 
 // RMSNorm of every query and key head and the rotation of its position:
 //   y = x * (1 / sqrt(mean(x^2) + eps)) * w
@@ -391,9 +441,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const RopeParams p) {
   const int pos = __ldg(p.pos + row);
   if (pos < 0) return;
   const T* x = static_cast<const T*>(p.x) + (size_t)row * p.x_stride + (size_t)(is_q ? 0 : p.n_head) * HD + l * E;
-  float v[BATCH][E];
+  RopeVec<T, E> raw[BATCH];
 #pragma unroll
-  for (int b = 0; b < BATCH; ++b) rope_load(x + (size_t)min(h0 + b * AT_ONCE, heads - 1) * HD, v[b]);
+  for (int b = 0; b < BATCH; ++b) raw[b].load(x + (size_t)min(h0 + b * AT_ONCE, heads - 1) * HD);
   if (pos >= p.n_pos) {
     if (lane == 0 && p.err) atomicExch(p.err, KERR_PAGES);
     return;
@@ -410,16 +460,22 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const RopeParams p) {
   }
   const float* norm = is_q ? p.q_norm : p.k_norm;
   float w[E];
-  if (norm) rope_load(norm + l * E, w);
+  if (norm) {
+    RopeVec<float, E> f;
+    f.load(norm + l * E);
+    f.get(w);
+  }
   T* out = is_q ? static_cast<T*>(p.q) + (size_t)row * p.q_stride : static_cast<T*>(p.k) + (size_t)row * p.k_stride;
   out += l * E;
 #pragma unroll
   for (int b = 0; b < BATCH; ++b) {
     const int h = h0 + b * AT_ONCE;
+    float v[E];
+    raw[b].get(v);
     if (norm) {
       float ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < E; ++i) ss = fmaf(v[b][i], v[b][i], ss);
+      for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const float mean = fmaf(ss, 1.0f / HD, p.eps);
@@ -428,21 +484,21 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const RopeParams p) {
       // (an infinite mean, or zero with no eps, has nothing to refine)
       if (!(mean > 0.0f) || isinf(mean)) scale = rsqrtf(mean);
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[b][i] = __fmul_rn(__fmul_rn(v[b][i], scale), w[i]);
+      for (int i = 0; i < E; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], scale), w[i]);
     }
     float o[E];
     if (HALVES) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const float other = __shfl_xor_sync(0xffffffffu, v[b][i], LANES / 2);
-        o[i] = l < LANES / 2 ? __fsub_rn(__fmul_rn(v[b][i], cs[i]), __fmul_rn(other, sn[i]))
-                             : __fadd_rn(__fmul_rn(other, sn[i]), __fmul_rn(v[b][i], cs[i]));
+        const float other = __shfl_xor_sync(0xffffffffu, v[i], LANES / 2);
+        o[i] = l < LANES / 2 ? __fsub_rn(__fmul_rn(v[i], cs[i]), __fmul_rn(other, sn[i]))
+                             : __fadd_rn(__fmul_rn(other, sn[i]), __fmul_rn(v[i], cs[i]));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < E; i += 2) {
-        o[i] = __fsub_rn(__fmul_rn(v[b][i], cs[i / 2]), __fmul_rn(v[b][i + 1], sn[i / 2]));
-        o[i + 1] = __fadd_rn(__fmul_rn(v[b][i], sn[i / 2]), __fmul_rn(v[b][i + 1], cs[i / 2]));
+        o[i] = __fsub_rn(__fmul_rn(v[i], cs[i / 2]), __fmul_rn(v[i + 1], sn[i / 2]));
+        o[i + 1] = __fadd_rn(__fmul_rn(v[i], sn[i / 2]), __fmul_rn(v[i + 1], cs[i / 2]));
       }
     }
     if (h < heads) rope_store(out + (size_t)h * HD, o);
