@@ -10,8 +10,11 @@
 #include "host.cuh"
 #include "kv4.cuh"
 #include "kv4_attn.cuh"
+#include "kv4_wide.cuh"
 
 using namespace fox;
+
+constexpr int KV4_WIDE_FROM = 16;
 
 static_assert(FOXCUDA_KV_PAGE == KV_PAGE, "the header's page size is the kernels'");
 
@@ -157,35 +160,28 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
 }
 
 // Two pieces of a tile for every CTA.
-template <int HD, int NT>
+template <int HD>
 static size_t kv4_work_bytes(int ctas) {
-  return (size_t)ctas * 2 * Kv4Attn<HD, NT>::PIECE_BYTES;
+  constexpr int wide = HD < 256 ? KV4_WIDE_PAIRS : 0;
+  return (size_t)ctas * 2 * std::max(wide, Kv4Attn<HD, 1>::PAIRS) * (HD + 4) * 4;
 }
 
 extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim, uint32_t table_stride) {
   if (table_stride <= KV4_WHOLE) return 0;  // no run is split between CTAs
   const int ctas = current_sms();
   switch (head_dim) {
-    case 64: return kv4_work_bytes<64, 1>(ctas);
-    case 128: return kv4_work_bytes<128, 1>(ctas);
-    case 256: return kv4_work_bytes<256, 1>(ctas);
+    case 64: return kv4_work_bytes<64>(ctas);
+    case 128: return kv4_work_bytes<128>(ctas);
+    case 256: return kv4_work_bytes<256>(ctas);
     default: return 0;
   }
 }
 
-template <typename T, int HD, int NT>
-static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
-  using A = Kv4Attn<HD, NT>;
-  const size_t smem = A::smem_bytes(p.c.n_seq);
-  static size_t marks[kMaxDevices] = {}, join_marks[kMaxDevices] = {};
-  cudaError_t e = opt_in_smem(kv4_attend_kernel<HD, T, NT>, smem, marks);
-  if (e != cudaSuccess) return e;
-  kv4_attend_kernel<HD, T, NT><<<p.ctas, A::NW * 32, smem, s>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if (p.c.table_stride <= KV4_WHOLE) return e;  // no run is split between CTAs
-  // the join of split runs, its launch overlapped with the attention
-  const int gqa = p.n_head / p.c.n_kv;
-  const size_t most = ((size_t)p.c.n_rows * gqa / A::PAIRS + p.c.n_seq) * p.c.n_kv * A::PAIRS;
+// The join of split runs, its launch overlapped with the attention.
+template <typename T, int HD, int PAIRS>
+static cudaError_t launch_kv4_join(const Kv4AttnParams& p, cudaStream_t s) {
+  static size_t marks[kMaxDevices] = {};
+  const size_t most = ((size_t)p.c.n_rows * (p.n_head / p.c.n_kv) / PAIRS + p.c.n_seq) * p.c.n_kv * PAIRS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)std::min<size_t>(most, (size_t)p.ctas * 8));
   cfg.blockDim = dim3(KV4_JOIN_WARPS * 32);
@@ -196,8 +192,32 @@ static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, cudaStream_t s) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if ((e = opt_in_smem(kv4_join_kernel<HD, T, NT>, cfg.dynamicSmemBytes, join_marks)) != cudaSuccess) return e;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, NT>, p);
+  cudaError_t e = opt_in_smem(kv4_join_kernel<HD, T, PAIRS>, cfg.dynamicSmemBytes, marks);
+  if (e != cudaSuccess) return e;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, PAIRS>, p);
+}
+
+template <typename T, int HD>
+static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, bool wide, cudaStream_t s) {
+  static size_t marks[2][kMaxDevices] = {};
+  const bool join = p.c.table_stride > KV4_WHOLE;  // else no run is split between CTAs
+  cudaError_t e;
+  if constexpr (HD < 256) {
+    if (wide) {
+      using A = Kv4Wide<HD>;
+      const size_t smem = A::smem_bytes(p.c.n_seq);
+      if ((e = opt_in_smem(kv4_wide_kernel<HD, T>, smem, marks[1])) != cudaSuccess) return e;
+      kv4_wide_kernel<HD, T><<<p.ctas, A::THREADS, smem, s>>>(p);
+      if ((e = cudaGetLastError()) != cudaSuccess || !join) return e;
+      return launch_kv4_join<T, HD, A::PAIRS>(p, s);
+    }
+  }
+  using A = Kv4Attn<HD, 1>;
+  const size_t smem = A::smem_bytes(p.c.n_seq);
+  if ((e = opt_in_smem(kv4_attend_kernel<HD, T, 1>, smem, marks[0])) != cudaSuccess) return e;
+  kv4_attend_kernel<HD, T, 1><<<p.ctas, A::NW * 32, smem, s>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess || !join) return e;
+  return launch_kv4_join<T, HD, A::PAIRS>(p, s);
 }
 
 extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, const void* q, size_t q_stride,
@@ -227,8 +247,10 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
   p.q = q; p.out = out; p.part = static_cast<float*>(workspace); p.q_stride = q_stride;
   p.n_head = (int)n_head; p.ctas = current_sms();
   p.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim);
+  // many rows a sequence: the tensor cores' 128-row tiles
+  const bool wide = c->head_dim < 256 && (size_t)c->n_rows * gqa >= (size_t)KV4_WIDE_FROM * c->n_seq;
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
-       return launch_kv4_attend<decltype(tag), hd.value, 1>(p, (cudaStream_t)stream);
+       return launch_kv4_attend<decltype(tag), hd.value>(p, wide, (cudaStream_t)stream);
      }), "kv4_attention launch");
   return FOXCUDA_OK;
 }

@@ -776,11 +776,10 @@ template <int HD>
 __host__ __device__ constexpr int kv4_join_smem(int n_seq) {
   return KV4_JOIN_WARPS * (HD + 2) * 4 + Kv4Line::bytes(n_seq);
 }
-template <int HD, typename T, int NT>
+template <int HD, typename T, int PAIRS>
 __global__ void __launch_bounds__(KV4_JOIN_WARPS * 32) kv4_join_kernel(const Kv4AttnParams p) {
-  using A = Kv4Attn<HD, NT>;
-  constexpr int PAIRS = A::PAIRS, E = HD / 32, JW = KV4_JOIN_WARPS;
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int E = HD / 32, JW = KV4_JOIN_WARPS, PART = HD + 4;
+  extern __shared__ __align__(128) uint8_t smem[];
   float* red = reinterpret_cast<float*>(smem);  // [JW][HD + 2]
   Kv4Line line;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gqa = p.n_head / p.c.n_kv;
@@ -808,7 +807,7 @@ __global__ void __launch_bounds__(KV4_JOIN_WARPS * 32) kv4_join_kernel(const Kv4
         out = static_cast<T*>(p.out) + ((size_t)(q.r0 + pr / gqa) * p.n_head + kv * gqa + pr % gqa) * HD;
 #pragma unroll 4
         for (int c = c0 + in_team; c <= c1; c += team)
-          sum.add(p.part + (((size_t)c * 2 + (c == c0)) * PAIRS + i) * A::PART);
+          sum.add(p.part + (((size_t)c * 2 + (c == c0)) * PAIRS + i) * PART);
       }
     }
     if (team > 1) {
