@@ -30,7 +30,7 @@
 
 namespace fox {
 
-constexpr int KV4_WIDE_PAIRS = 128, KV4_WIDE_FLUSH = 4;
+constexpr int KV4_WIDE_PAIRS = 128, KV4_WIDE_FLUSH = 8;
 
 template <int HD>
 struct Kv4Wide {
@@ -51,7 +51,7 @@ struct Kv4Wide {
   static constexpr int RAW = 3, PAR = 4;  // pages loaded ahead; pages whose parameters are kept
   // shared memory
   static constexpr int Q_AT = 0, K_AT = Q_AT + 2 * G * QTILE, V_AT = K_AT + 2 * G * TILE, RAW_AT = V_AT + 2 * G * TILE;
-  static constexpr int PAR_AT = RAW_AT + RAW * PAGE_BYTES, PAR_BYTES = 2 * KV_PAGE * G * 8;  // K's, then V's (d / 2, m + 7.5 d)
+  static constexpr int PAR_AT = RAW_AT + RAW * PAGE_BYTES, PAR_BYTES = 2 * KV_PAGE * G * 8;  // [K, V][group][d / 2, m + 7.5 d][position] floats
   static constexpr int EX_AT = PAR_AT + PAR * PAR_BYTES;                                    // the sharing threads' exchange: [SHARE][PAIRS] float4
   static constexpr int LINE_AT = EX_AT + SOFT * 16;
   static size_t smem_bytes(int n_seq) { return LINE_AT + Kv4Line::bytes(n_seq); }
@@ -69,15 +69,27 @@ struct Kv4WideBars {
 FOX_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Bounded, and at once when another wait of the CTA has given up.
+// Bounded, and at once when another wait of the CTA has given up. A poll may
+// sleep in the barrier's unit for up to 20 us, so that the waiting roles leave
+// the schedulers to the working ones.
 FOX_DEV bool kv4_wait(Kv4WideBars& b, uint64_t* bar, unsigned parity) {
-  for (int i = 0; i < (1 << 20); ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
+  for (int i = 0; i < (1 << 16); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
     if (*reinterpret_cast<volatile int*>(&b.dead)) return false;
-    if (i >= 64) __nanosleep(128);
   }
   *reinterpret_cast<volatile int*>(&b.dead) = 1;
   return false;
+}
+// The same by a warp. Every lane polls: one polling for the others was slower
+// by a quarter of the kernel's time.
+FOX_DEV bool kv4_warp_wait(Kv4WideBars& b, uint64_t* bar, unsigned parity) {
+  return __all_sync(0xffffffffu, kv4_wait(b, bar, parity));
 }
 FOX_DEV void mma_f16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   const uint32_t z = 0;
@@ -120,6 +132,40 @@ FOX_DEV bool kv4_any(bool x) {
   return r != 0;
 }
 FOX_DEV void kv4_soft_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
+
+FOX_DEV bool kv4_elect() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+
+// Two floats in one register pair: one instruction for both.
+typedef unsigned long long f32x2;
+FOX_DEV f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+FOX_DEV float2 unpack2(f32x2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+FOX_DEV f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+FOX_DEV f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+FOX_DEV f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 
 // 8 codes as fp16 2 c - 15, in the order (0, 4), (1, 5), (2, 6), (3, 7).
 FOX_DEV void kv4_centred(uint32_t x, uint32_t (&h)[4]) {
@@ -272,15 +318,15 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.q_full);
       }
-      float o[OWN], mx = -INFINITY, l = 0.0f, mo[G], big = 0x1p-24f;
+      float o[OWN], mx = -INFINITY, big = 0x1p-24f;
+      f32x2 l = 0, mo[G];  // of every other position
 #pragma unroll
       for (int i = 0; i < OWN; ++i) o[i] = 0.0f;
 #pragma unroll
-      for (int g = 0; g < G; ++g) mo[g] = 0.0f;
+      for (int g = 0; g < G; ++g) mo[g] = 0;
       int since = 0;  // pages in tensor memory's sums
       auto take_sums = [&]() {  // O of the pages up to j - 1, into the registers
-        if (since && !kv4_wait(bars, &bars.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
+        if (since && !kv4_warp_wait(bars, &bars.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) ok = false;
         if (!since || !ok) return;
         tc_fence_after();
 #pragma unroll
@@ -297,12 +343,13 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
       for (int page = r.first; page < r.last; ++page, ++j) {
         const int b = j & 1, pos0 = page * KV_PAGE + share * A::POS;
         const unsigned ph = (j >> 1) & 1;
-        ok = kv4_wait(bars, &bars.k_full[b], ph) && kv4_wait(bars, &bars.v_full[b], ph) && kv4_wait(bars, &bars.s_full[b], ph);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = kv4_warp_wait(bars, &bars.k_full[b], ph) && kv4_warp_wait(bars, &bars.v_full[b], ph) &&
+             kv4_warp_wait(bars, &bars.s_full[b], ph);
         tc_fence_after();
-        // this thread's positions' parameters: K's, then V's
-        const float2* kp = reinterpret_cast<const float2*>(smem + A::PAR_AT + (j & 3) * A::PAR_BYTES) + share * A::POS * G;
-        const float2* vp = kp + KV_PAGE * G;
+        // this thread's positions' parameters: K's, then V's; four at once
+        const float* kp = reinterpret_cast<const float*>(smem + A::PAR_AT + (j & 3) * A::PAR_BYTES) + share * A::POS;
+        const float* vp = kp + 2 * G * KV_PAGE;
+        auto par4 = [](const float* p) { return *reinterpret_cast<const ulonglong2*>(p); };
         const uint32_t s_at = tmem + lanes + b * A::S_COLS;
         const bool absent = bars.absent[j & 3], edge = absent || page * KV_PAGE + KV_PAGE - 1 > lim_min;
         const uint32_t mine = tmem + lanes + A::SCORE_COL + share * A::POS;
@@ -317,19 +364,29 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
             for (int g = 0; g < G; ++g) TmemLd<16>::run(s_at + g * 64 + share * A::POS + c, d[g]);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float s;
-              if constexpr (G == 2) {
-                const float4 k = *reinterpret_cast<const float4*>(kp + 2 * (c + i));
-                s = fmaf(f, fmaf(k.x, __uint_as_float(d[0][i]), k.z * __uint_as_float(d[G - 1][i])),
-                         fmaf(k.y, qs[0], k.w * qs[G - 1]));
-              } else {
-                const float2 k = kp[c + i];
-                s = fmaf(f, k.x * __uint_as_float(d[0][i]), k.y * qs[0]);
+            for (int i = 0; i < 16; i += 4) {
+              f32x2 prod[2], off[2];
+#pragma unroll
+              for (int g = 0; g < G; ++g) {
+                const ulonglong2 dd = par4(kp + 2 * g * KV_PAGE + c + i), mm = par4(kp + (2 * g + 1) * KV_PAGE + c + i);
+                const f32x2 q2 = pack2(qs[g], qs[g]), dk[2] = {dd.x, dd.y}, mk[2] = {mm.x, mm.y};
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const f32x2 x = pack2(__uint_as_float(d[g][i + 2 * k]), __uint_as_float(d[g][i + 2 * k + 1]));
+                  prod[k] = g ? fma2(dk[k], x, prod[k]) : mul2(dk[k], x);
+                  off[k] = g ? fma2(mk[k], q2, off[k]) : mul2(mk[k], q2);
+                }
               }
-              if (at_edge.value && (absent || pos0 + c + i > lim)) s = -INFINITY;
-              top = fmaxf(top, s);
-              d[0][i] = __float_as_uint(s);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                float2 s = unpack2(fma2(pack2(f, f), prod[k], off[k]));
+                const int at = pos0 + c + i + 2 * k;
+                if (at_edge.value && (absent || at > lim)) s.x = -INFINITY;
+                if (at_edge.value && (absent || at + 1 > lim)) s.y = -INFINITY;
+                top = fmaxf(top, fmaxf(s.x, s.y));
+                d[0][i + 2 * k] = __float_as_uint(s.x);
+                d[0][i + 2 * k + 1] = __float_as_uint(s.y);
+              }
             }
             tmem_st16(mine + c, d[0]);
           }
@@ -353,9 +410,9 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
           const float al = m == -INFINITY ? 1.0f : exp2_approx(mx - m), all = al * (big / to);
           mx = m;
           big = to;
-          l *= al;
+          l = mul2(l, pack2(al, al));
 #pragma unroll
-          for (int g = 0; g < G; ++g) mo[g] *= al;
+          for (int g = 0; g < G; ++g) mo[g] = mul2(mo[g], pack2(al, al));
 #pragma unroll
           for (int i = 0; i < OWN; ++i) o[i] *= all;
         }
@@ -367,34 +424,42 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
             uint32_t s[16], hi[G][8], lo[G][8];
             TmemLd<16>::run(mine + c, s);
             tmem_wait_ld();
+            const f32x2 below = pack2(-base, -base), norm2 = pack2(norm, norm);
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float v[G][2];
+            for (int i = 0; i < 16; i += 4) {
+              f32x2 w[2], wn[2];
+              bool hidden[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)  // whatever the position holds
+                hidden[k] = at_edge.value && __uint_as_float(s[i + k]) == -INFINITY;
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const float sc = __uint_as_float(s[i + k]), w = exp2_approx(sc - base), wn = w * norm;
-                const bool hidden = at_edge.value && sc == -INFINITY;  // whatever the position holds
-                float2 dm[G];
-                if constexpr (G == 2) {
-                  const float4 x = *reinterpret_cast<const float4*>(vp + 2 * (c + i + k));
-                  dm[0] = make_float2(x.x, x.y);
-                  dm[G - 1] = make_float2(x.z, x.w);
-                } else {
-                  dm[0] = vp[c + i + k];
-                }
-                l += w;
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                  v[g][k] = hidden ? 0.0f : wn * dm[g].x;
-                  mo[g] = fmaf(w, hidden ? 0.0f : dm[g].y, mo[g]);
-                }
+                const float2 x = unpack2(add2(pack2(__uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1])), below));
+                w[k] = pack2(exp2_approx(x.x), exp2_approx(x.y));
+                wn[k] = mul2(w[k], norm2);
+                l = add2(l, w[k]);
               }
 #pragma unroll
               for (int g = 0; g < G; ++g) {
-                const float h0 = __uint_as_float(__float_as_uint(v[g][0]) & 0xffffe000u);
-                const float h1 = __uint_as_float(__float_as_uint(v[g][1]) & 0xffffe000u);
-                hi[g][i / 2] = half2_bits(__floats2half2_rn(h0, h1));
-                lo[g][i / 2] = half2_bits(__floats2half2_rn(v[g][0] - h0, v[g][1] - h1));
+                const ulonglong2 dd = par4(vp + 2 * g * KV_PAGE + c + i), mm = par4(vp + (2 * g + 1) * KV_PAGE + c + i);
+                const f32x2 dk[2] = {dd.x, dd.y};
+                f32x2 mk[2] = {mm.x, mm.y};
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  float2 v = unpack2(mul2(wn[k], dk[k]));
+                  if (at_edge.value) {
+                    float2 m = unpack2(mk[k]);
+                    if (hidden[2 * k]) v.x = m.x = 0.0f;
+                    if (hidden[2 * k + 1]) v.y = m.y = 0.0f;
+                    mk[k] = pack2(m.x, m.y);
+                  }
+                  mo[g] = fma2(w[k], mk[k], mo[g]);
+                  const float h0 = __uint_as_float(__float_as_uint(v.x) & 0xffffe000u);
+                  const float h1 = __uint_as_float(__float_as_uint(v.y) & 0xffffe000u);
+                  const float2 rest = unpack2(add2(pack2(v.x, v.y), pack2(-h0, -h1)));
+                  hi[g][i / 2 + k] = half2_bits(__floats2half2_rn(h0, h1));
+                  lo[g][i / 2 + k] = half2_bits(__floats2half2_rn(rest.x, rest.y));
+                }
               }
             }
 #pragma unroll
@@ -414,14 +479,16 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
       }
       take_sums();
       // the shares of l and the offsets, and the result
-      ex[share * PAIRS] = make_float4(l, mo[0], mo[G - 1], 0.0f);
+      {
+        const float2 a = unpack2(l), m0 = unpack2(mo[0]), m1 = unpack2(mo[G - 1]);
+        ex[share * PAIRS] = make_float4(a.x + a.y, m0.x + m0.y, m1.x + m1.y, 0.0f);
+      }
       if (kv4_any(!ok)) { ok = false; break; }
-      float off = 0.0f;
-      l = 0.0f;
+      float off = 0.0f, total = 0.0f;
 #pragma unroll
       for (int k = 0; k < A::SHARE; ++k) {
         const float4 e = ex[k * PAIRS];
-        l += e.x;
+        total += e.x;
         off += share * G / A::SHARE ? e.z : e.y;
       }
       const float unit = big / KV4_WEIGHT;
@@ -430,12 +497,12 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         T* out = static_cast<T*>(p.out) + ((size_t)(r.x.q.r0 + row) * p.n_head + head) * HD + share * OWN;
         float* dst = p.part + (((size_t)blockIdx.x * 2 + r.begins) * PAIRS + pair) * A::PART;
         const bool whole = r.begins && r.ends;
-        if (!whole && share == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx, l);
+        if (!whole && share == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx, total);
 #pragma unroll
         for (int i = 0; i < OWN; i += 4) {
           const float4 v = make_float4(fmaf(o[i], unit, off), fmaf(o[i + 1], unit, off), fmaf(o[i + 2], unit, off),
                                        fmaf(o[i + 3], unit, off));
-          if (whole) kv4_store4(out + i, kv4_quotient(v, l));
+          if (whole) kv4_store4(out + i, kv4_quotient(v, total));
           else *reinterpret_cast<float4*>(dst + 4 + share * OWN + i) = v;
         }
       }
@@ -457,14 +524,16 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         const uint8_t* raw = smem + A::RAW_AT + (j % 3) * A::PAGE_BYTES + side * A::BB;
         const int at = __ldg(p.c.table + (size_t)r.x.seq * p.c.table_stride + page);
         const bool absent = (unsigned)at >= (unsigned)p.c.n_pages;
-        ok = kv4_wait(bars, &bars.raw_full[j % 3], (j / 3) & 1) && (j < 2 || kv4_wait(bars, &freed[b], ((j - 2) >> 1) & 1));
-        ok = __all_sync(0xffffffffu, ok);
+        ok = kv4_warp_wait(bars, &bars.raw_full[j % 3], (j / 3) & 1) &&
+             (j < 2 || kv4_warp_wait(bars, &freed[b], ((j - 2) >> 1) & 1));
         if (!ok) break;
-        float2* par = reinterpret_cast<float2*>(smem + A::PAR_AT + (j & 3) * A::PAR_BYTES) + side * KV_PAGE * G;
-        auto param = [&](int i) {  // position i / G, group i % G: its d
-          const float2 dm = __half22float2(reinterpret_cast<const __half2*>(raw + kv4_codes_bytes(HD))[i]);
-          const bool seen = !absent && i / G <= left;  // else whatever the memory held
-          par[i] = seen ? make_float2(0.5f * dm.x, fmaf(7.5f, dm.x, dm.y)) : make_float2(0.0f, 0.0f);
+        float* par = reinterpret_cast<float*>(smem + A::PAR_AT + (j & 3) * A::PAR_BYTES) + side * 2 * G * KV_PAGE;
+        auto param = [&](int i) {  // position i % 64, group i / 64: its d
+          const int pos = i % KV_PAGE, g = i / KV_PAGE;
+          const float2 dm = __half22float2(reinterpret_cast<const __half2*>(raw + kv4_codes_bytes(HD))[pos * G + g]);
+          const bool seen = !absent && pos <= left;  // else whatever the memory held
+          par[2 * g * KV_PAGE + pos] = seen ? 0.5f * dm.x : 0.0f;
+          par[(2 * g + 1) * KV_PAGE + pos] = seen ? fmaf(7.5f, dm.x, dm.y) : 0.0f;
           return seen ? dm.x : 0.0f;
         };
         if (!side) {
@@ -522,8 +591,10 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
       }
       u = r.next;
     }
-  } else if (lane == 0) {
-    // ---- the loads and the products
+  } else {
+    // ---- the loads and the products. The whole warp walks (its values stay in
+    // uniform registers, which the instructions want them in), one lane issues.
+    const bool leader = kv4_elect();
     constexpr uint32_t IDESC = (1u << 4) | ((64u >> 3) << 17) | ((uint32_t)(PAIRS >> 4) << 24);  // fp32 sums of fp16, both K-major
     int pages = 0;  // of the whole stretch
     for (int u = a0; u < a1;) {
@@ -544,8 +615,8 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
       const int page = kv4_page(p.c, lr.x.seq, lp * KV_PAGE);
       uint64_t* bar = &bars.raw_full[loaded % 3];
       // an absent page is not read: its positions count for nothing
-      mbar_arrive_expect_tx(bar, page >= 0 ? A::PAGE_BYTES : 0);
-      if (page >= 0)
+      if (leader) mbar_arrive_expect_tx(bar, page >= 0 ? A::PAGE_BYTES : 0);
+      if (leader && page >= 0)
         bulk_g2s(smem + A::RAW_AT + (loaded % 3) * A::PAGE_BYTES, kv4_block(p.c, page, lr.x.kv, 0, A::BB), A::PAGE_BYTES, bar);
       ++lp;
       ++loaded;
@@ -557,17 +628,20 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
     auto pv = [&](int i) {  // O += P . V of page i
       const int b = i & 1;
       const unsigned ph = (i >> 1) & 1;
-      ok = ok && kv4_wait(bars, &bars.v_full[b], ph) && kv4_wait(bars, &bars.p_full[b], ph);
+      ok = ok && kv4_warp_wait(bars, &bars.v_full[b], ph) && kv4_warp_wait(bars, &bars.p_full[b], ph);
       if (!ok) return;
       tc_fence_after();
       const uint32_t add = *reinterpret_cast<volatile int*>(&bars.fresh[b]) ? 0u : 1u;
+      if (leader) {
+        const uint64_t v = umma_desc(v0 + b * G * A::TILE, A::LBO, A::SBO);
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int s = 0; s < 8; ++s)  // hi, then lo; 16 positions each
-          mma_f16_ts(tmem + A::O_COL + g * 64, tmem + b * A::S_COLS + g * 64 + s * 8,
-                     umma_desc(v0 + (b * G + g) * A::TILE + (s & 3) * 2 * A::LBO, A::LBO, A::SBO), IDESC, s ? 1u : add);
-      mma_commit(&bars.pv_done[b]);
+          for (int s = 0; s < 8; ++s)  // hi, then lo; 16 positions each
+            mma_f16_ts(tmem + A::O_COL + g * 64, tmem + b * A::S_COLS + g * 64 + s * 8,
+                       v + ((g * A::TILE + (s & 3) * 2 * A::LBO) >> 4), IDESC, s ? 1u : add);
+        mma_commit(&bars.pv_done[b]);
+      }
       done = i;
       if (loaded < pages) load();  // the slot of page i: its codes have been unpacked
     };
@@ -577,20 +651,23 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         const int b = j & 1;
         if (page == r.first) {  // the queries change once the last run's sums are taken
           if (j) pv(j - 1);
-          ok = ok && kv4_wait(bars, &bars.q_full, runs & 1);
+          ok = ok && kv4_warp_wait(bars, &bars.q_full, runs & 1);
           ++runs;
         }
         // (the buffer's last weights were used by the products of page j - 2)
-        ok = ok && kv4_wait(bars, &bars.k_full[b], (j >> 1) & 1) && (j < 2 || kv4_wait(bars, &bars.pv_done[b], ((j - 2) >> 1) & 1));
+        ok = ok && kv4_warp_wait(bars, &bars.k_full[b], (j >> 1) & 1) && (j < 2 || kv4_warp_wait(bars, &bars.pv_done[b], ((j - 2) >> 1) & 1));
         if (!ok) break;
         tc_fence_after();
+        if (leader) {
+          const uint64_t q = umma_desc(q0, A::QLBO, A::QSBO), k = umma_desc(k0 + b * G * A::TILE, A::LBO, A::SBO);
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+          for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int s = 0; s < 8; ++s)  // hi, then lo; 16 dimensions each
-            mma_f16(tmem + b * A::S_COLS + g * 64, umma_desc(q0 + ((s >> 2) * G + g) * A::QTILE + (s & 3) * 2 * A::QLBO, A::QLBO, A::QSBO),
-                    umma_desc(k0 + (b * G + g) * A::TILE + (s & 3) * 2 * A::LBO, A::LBO, A::SBO), IDESC, s ? 1u : 0u);
-        mma_commit(&bars.s_full[b]);
+            for (int s = 0; s < 8; ++s)  // hi, then lo; 16 dimensions each
+              mma_f16(tmem + b * A::S_COLS + g * 64, q + ((((s >> 2) * G + g) * A::QTILE + (s & 3) * 2 * A::QLBO) >> 4),
+                      k + ((g * A::TILE + (s & 3) * 2 * A::LBO) >> 4), IDESC, s ? 1u : 0u);
+          mma_commit(&bars.s_full[b]);
+        }
         if (page > r.first) pv(j - 1);
       }
       u = r.next;
