@@ -14,7 +14,16 @@
 
 using namespace fox;
 
-constexpr int KV4_WIDE_FROM = 16;
+// Attention takes the 5th-generation tensor cores' tiles from this many (row,
+// head) pairs a sequence and KV head on: their time hardly depends on the rows.
+// 4 sequences of 16384 positions, 8 KV heads of 128: 32 pairs 120 us either way,
+// 48 pairs 170 us narrow and 121 wide, 128 pairs 423 and 130; of 64: 32 pairs 77
+// and 83, 48 pairs 110 and 84.
+constexpr int KV4_WIDE_FROM = 48;
+// Where no run is split, a tile has one SM for its pages, so there must also be
+// this many pairs an SM: one sequence of 1000 positions, 128 pairs for each of 8
+// KV heads, 18 us narrow and 42 wide; 16 of 512, 48 pairs, 41 and 27.
+constexpr int KV4_WIDE_FILL = 32;
 
 static_assert(FOXCUDA_KV_PAGE == KV_PAGE, "the header's page size is the kernels'");
 
@@ -248,7 +257,8 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
   p.n_head = (int)n_head; p.ctas = current_sms();
   p.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim);
   // many rows a sequence: the tensor cores' 128-row tiles
-  const bool wide = c->head_dim < 256 && (size_t)c->n_rows * gqa >= (size_t)KV4_WIDE_FROM * c->n_seq;
+  const bool wide = c->head_dim < 256 && (size_t)c->n_rows * gqa >= (size_t)KV4_WIDE_FROM * c->n_seq &&
+                    (c->table_stride > KV4_WHOLE || (size_t)c->n_rows * n_head >= (size_t)KV4_WIDE_FILL * p.ctas);
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
        return launch_kv4_attend<decltype(tag), hd.value>(p, wide, (cudaStream_t)stream);
      }), "kv4_attention launch");

@@ -77,6 +77,7 @@ struct Kv4WideBars {
   float k_unit[4], v_unit[4];           // what 1 stands for in the page's operands
   unsigned v_bad[4][4];                 // positions whose V is not finite: [group][half of the page]
   int absent[8];                        // the block table names no page
+  unsigned seen[2][2][4];               // K's and V's warps: sizes in their parameters (1 not small, 2 large), 4 gave up
   int dead;                             // a wait gave up
 };
 
@@ -120,18 +121,16 @@ FOX_DEV void tmem_st8(uint32_t a, const uint32_t (&v)[8]) {
                : "memory");
 }
 FOX_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// Whether any of a role's N threads says so, and their barrier.
-template <int BAR, int N>
-FOX_DEV bool kv4_any(bool x) {
+// Whether any of the 256 weight-forming threads says so (their barrier).
+FOX_DEV bool kv4_soft_any(bool x) {
   uint32_t r;
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 256, p;\n selp.u32 %0, 1, 0, q;\n}"
       : "=r"(r)
-      : "r"((uint32_t)x), "n"(BAR), "n"(N)
+      : "r"((uint32_t)x)
       : "memory");
   return r != 0;
 }
-FOX_DEV bool kv4_soft_any(bool x) { return kv4_any<1, 256>(x); }
 FOX_DEV void kv4_soft_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 
 FOX_DEV bool kv4_elect() {
@@ -161,9 +160,12 @@ FOX_DEV void kv4_split(float x, __half* hi, __half* lo) {
   *hi = __float2half_rn(x);
   *lo = __float2half_rn(x - __half2float(*hi));
 }
-// A page's operands are its fp16 parameters times small integers, so multiples
-// of 2^-24: nothing is lost below. Where one could pass 2^15, all are scaled.
-constexpr float KV4_SHRINK = 1.0f / 128.0f;
+// What a page's operands are scaled by, of the size |2 m + 15 d| + 15 |d| of its
+// largest group. Unscaled they are multiples of 2^-24, so that nothing is lost;
+// but large ones must stay below 2^16, and pages of small ones leave fp16's
+// subnormal numbers, for which the products' sums keep fewer bits.
+constexpr float KV4_LARGE = 32768.0f, KV4_SMALL = 1.0f / 16.0f;
+FOX_DEV float kv4_scale_of(int level) { return level == 0 ? 1.0f / 128.0f : level == 1 ? 1.0f : 65536.0f; }
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const Kv4AttnParams p) {
@@ -382,13 +384,20 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
           for (int i = 0; i < OWN; ++i) o[i] *= all;
         }
         if (tid == 0) bars.fresh[b] = since == 0;
-        // weights up to 2^7 by KV4_WEIGHT, 2^15 at most
-        const float base = 8.0f - (mx == -INFINITY ? 0.0f : mx);
-        static_assert(KV4_WEIGHT == 256.0f && KV4_SLACK == 7.0f, "2^8, and 2^7 of slack");
+        // Weights are scaled by 2^7, out of fp16's small numbers; with the slack
+        // they reach 2^14. The product is rounded before the sum, as the
+        // reference point was, so that the largest of scores of any size has a
+        // weight of 1 to 2^14: a fused one differed from it by more than 2^7
+        // from scores of 10^8 on. (7 - mx, rounded, is off by less than 4 where
+        // scores are that coarse, and those above mx by no more than the slack
+        // are then equal to it.)
+        const float base = 7.0f - (mx == -INFINITY ? 0.0f : mx);
+        static_assert(KV4_SLACK == 7.0f, "2^14, and not fp16's 2^16");
         uint32_t hi[A::POS / 2], lo[A::POS / 2];
 #pragma unroll
         for (int i = 0; i < A::POS; i += 2) {
-          const float w0 = exp2_approx(fmaf(__uint_as_float(d[i]), fj, base)), w1 = exp2_approx(fmaf(__uint_as_float(d[i + 1]), fj, base));
+          const float w0 = exp2_approx(__fadd_rn(__fmul_rn(__uint_as_float(d[i]), fj), base));
+          const float w1 = exp2_approx(__fadd_rn(__fmul_rn(__uint_as_float(d[i + 1]), fj), base));
           l += w0 + w1;
           const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
           hi[i / 2] = half2_bits(__floats2half2_rn(h0, h1));
@@ -444,18 +453,22 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
     }
     if (!ok && tid == 0 && p.c.err) atomicExch(p.c.err, KERR_WAIT);
   } else if (warp < MMA_WARP) {
-    // ---- a page's operands
+    // ---- a page's operands. Their loops stay rolled: four roles share a
+    // scheduler's instruction cache, and copies of the bodies cost 6 %.
     const int side = warp < A::K_WARP, t0 = tid - (side ? A::V_WARP : A::K_WARP) * 32;  // K 0, V 1
     constexpr int NK = (MMA_WARP - A::K_WARP) * 32, NV = (A::K_WARP - A::V_WARP) * 32, EACH = (KV_PAGE * G + NK - 1) / NK;
     static_assert(KV_PAGE * G <= NV, "a thread for each position and group of V");
     const int n = side ? NV : NK;
     uint64_t* freed = side ? bars.pv_done : bars.s_full;  // the products that used the buffers last
-    auto any = [&](bool x) { return side ? kv4_any<3, NV>(x) : kv4_any<2, NK>(x); };
+    auto sync = [&]() {
+      if (side) asm volatile("barrier.cta.sync 3, %0;" ::"n"(NV) : "memory");
+      else asm volatile("barrier.cta.sync 2, %0;" ::"n"(NK) : "memory");
+    };
     int j = 0;
     bool ok = true;
     for (int u = a0; u < a1 && ok;) {
       const Part r = part_at(u);
-      bool shrink = false;  // for good within a run: V's sums need one scale
+      int level = 2;  // V's only falls within a run: its sums have one scale
       for (int page = r.first; page < r.last; ++page, ++j) {
         const int b = j & 1, left = r.lim_max - page * KV_PAGE;  // positions 0 .. left of the page are seen
         const uint8_t* raw = smem + A::RAW_AT + (j % A::RAW) * A::PAGE_BYTES + side * A::BB;
@@ -466,7 +479,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         // the parameters: position i % 64 of group i / 64; zero where the
         // position is nobody's, whatever the memory held
         float d[EACH], off[EACH];
-        bool large = false;
+        float top = 0.0f;
 #pragma unroll
         for (int k = 0; k < EACH; ++k) {
           const int i = t0 + k * n, pos = i % KV_PAGE, g = i / KV_PAGE;
@@ -478,13 +491,14 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
             off[k] = fmaf(15.0f, dm.x, 2.0f * dm.y);
             const float size = fmaf(15.0f, fabsf(d[k]), fabsf(off[k]));
             bad = !(size < 1e30f);  // not finite
-            large |= size > 32768.0f && !bad;
-            if (side && bad) d[k] = off[k] = 0.0f;
+            if (!bad) top = fmaxf(top, size);
+            else if (side) d[k] = off[k] = 0.0f;
           }
           const unsigned bads = __ballot_sync(0xffffffffu, bad);
           if (side && k == 0 && lane == 0) bars.v_bad[j & 3][warp & 3] = bads;
         }
-        auto store = [&](float sc) {
+        auto store = [&]() {
+          const float sc = kv4_scale_of(level);
 #pragma unroll
           for (int k = 0; k < EACH; ++k) {
             const int i = t0 + k * n, pos = i % KV_PAGE, g = i / KV_PAGE;
@@ -505,15 +519,22 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
           }
           if (t0 == 0) (side ? bars.v_unit : bars.k_unit)[j & 3] = 0.5f / sc;
         };
-        if (ok) store(1.0f);
-        if (any(!ok || large || shrink)) {
-          if (any(!ok)) { ok = false; break; }
-          shrink = side;
-          store(KV4_SHRINK);
-          any(false);
+        // as the last page's, until all have been seen
+        if (ok) store();
+        const unsigned seen = (__any_sync(0xffffffffu, top >= KV4_SMALL) ? 1u : 0u) | (__any_sync(0xffffffffu, top > KV4_LARGE) ? 2u : 0u);
+        if (lane == 0) bars.seen[side][b][warp & 3] = ok ? seen : 4u;
+        sync();
+        unsigned all = 0;
+        for (int k = 0; k < n / 32; ++k) all |= bars.seen[side][b][k];
+        if (all & 4) { ok = false; break; }
+        const int now = min(side ? level : 2, all & 2 ? 0 : all & 1 ? 1 : 2);
+        if (now != level) {
+          level = now;
+          store();
+          sync();
         }
         if (!side) {
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < (KV_PAGE * 4 + NK - 1) / NK; ++k) {  // position i / 4, 16 dimensions of every group
             const int i = t0 + k * NK;
             if (i >= KV_PAGE * 4) break;
@@ -535,7 +556,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
             }
           }
         } else {
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < G; ++k) {  // 4 dimensions (g) of a block of 32, 8 positions
             const int i = t0 + k * NV, g = i & 7, blk = i / 8 % (2 * G), chunk = i / (16 * G);
             const uint4 d4 = *reinterpret_cast<const uint4*>(dd + blk / 2 * KV_PAGE + chunk * 8);
@@ -588,14 +609,18 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         lr = part_at(lu);
         lp = lr.first;
       }
-      next = kv4_page(p.c, lr.x.seq, lp * KV_PAGE);
+      next = __ldg(p.c.table + (size_t)lr.x.seq * p.c.table_stride + lp);  // looked at when it is used
     };
     auto load = [&]() {
       uint64_t* bar = &bars.raw_full[loaded % A::RAW];
-      // an absent page is not read: its positions count for nothing
-      if (leader) bars.absent[loaded & 7] = next < 0;
-      if (leader) mbar_arrive_expect_tx(bar, next >= 0 ? A::PAGE_BYTES : 0);
-      if (leader && next >= 0)
+      // a page outside the cache is not read: its positions count for nothing
+      const bool there = (unsigned)next < (unsigned)p.c.n_pages;
+      if (leader) {
+        bars.absent[loaded & 7] = !there;
+        mbar_arrive_expect_tx(bar, there ? A::PAGE_BYTES : 0);
+        if (!there && p.c.err) atomicExch(p.c.err, KERR_PAGES);
+      }
+      if (leader && there)
         bulk_g2s(smem + A::RAW_AT + (loaded % A::RAW) * A::PAGE_BYTES, kv4_block(p.c, next, lr.x.kv, 0, A::BB), A::PAGE_BYTES, bar);
       ++lp;
       ++loaded;
