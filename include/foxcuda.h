@@ -215,16 +215,17 @@ typedef struct {
 } foxcuda_kv4;
 size_t         foxcuda_kv4_block_bytes(uint32_t head_dim);   /* 0: not covered */
 /* Quantises each row's K and V heads into its position. k and v are FOXCUDA_F32
- * or FOXCUDA_F16 rows of n_head_kv * head_dim values. */
+ * or FOXCUDA_F16 rows of n_head_kv * head_dim values. Where two sequences'
+ * tables share a page and both write one position of it, either's bytes remain. */
 foxcuda_status foxcuda_kv4_write(const foxcuda_kv4 *c, int ggml_type, const void *k, size_t k_stride,
                                  const void *v, size_t v_stride, void *stream);
 /* The K and V values of each row's position, to rows of n_head_kv * head_dim
- * FOXCUDA_F32 or FOXCUDA_F16 values. */
+ * FOXCUDA_F32 or FOXCUDA_F16 values that do not overlap. */
 foxcuda_status foxcuda_kv4_read(const foxcuda_kv4 *c, int ggml_type, void *k, void *v, void *stream);
 /* Each row's n_head query heads over positions 0..its own of its sequence
  * (upstream attention_heads, src/forward.c:222-257, for many rows): q and out
  * are rows of n_head * head_dim FOXCUDA_F32 or FOXCUDA_F16 values, q's
- * q_stride elements apart. n_head / n_head_kv is 1, 2, 4 or 8; scale
+ * q_stride elements apart; they must not overlap. n_head / n_head_kv is 1, 2, 4 or 8; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). The sums and softmax
  * statistics are fp32. The same call gives the same bits; a row's sums are
  * split where an even division of the call's pages falls, so its last bits

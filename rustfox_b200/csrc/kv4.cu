@@ -30,6 +30,9 @@ static_assert(FOXCUDA_KV_PAGE == KV_PAGE, "the header's page size is the kernels
 static bool kv4_hd_ok(uint32_t hd) { return hd == 64 || hd == 128 || hd == 256; }
 static bool kv4_type_ok(int t) { return t == T_F32 || t == T_F16; }
 static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
 static bool stride_ok(size_t stride, size_t row, int type) {
   return stride >= row && stride * (type == T_F32 ? 4 : 2) % 16 == 0 && stride <= ((size_t)1 << 32);
 }
@@ -112,6 +115,8 @@ extern "C" foxcuda_status foxcuda_kv4_read(const foxcuda_kv4* c, int type, void*
   if (st || none) return st;
   if (!k || !v) return fail(FOXCUDA_ERR_ARG, "kv4_read: null pointer");
   if (!aligned16(k) || !aligned16(v)) return fail(FOXCUDA_ERR_ARG, "kv4_read: rows must be 16-byte aligned");
+  const size_t bytes = (size_t)c->n_rows * c->n_head_kv * c->head_dim * (type == T_F32 ? 4 : 2);
+  if (overlap(k, bytes, v, bytes)) return fail(FOXCUDA_ERR_ARG, "kv4_read: the outputs overlap");
   p.k = k; p.v = v;
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
        return by_rows<hd.value>(p.c, [&](auto rows, unsigned grid) {
@@ -246,6 +251,9 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) ||
       !stride_ok(q_stride, (size_t)n_head * c->head_dim, type))
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: rows and workspace must be 16-byte aligned, rows at least a row apart");
+  const size_t size = type == T_F32 ? 4 : 2, row = (size_t)n_head * c->head_dim;
+  if (overlap(q, ((c->n_rows - 1) * q_stride + row) * size, out, c->n_rows * row * size))
+    return fail(FOXCUDA_ERR_ARG, "kv4_attention: q and out overlap");
   // tiles of at least 4 (row, head) pairs, each with every page of its sequence
   const double units = ((double)c->n_rows * gqa / 4 + c->n_seq) * c->n_head_kv * ((double)c->table_stride + KV4_HEAD);
   if (units >= 2147483648.0)

@@ -180,3 +180,30 @@ def test_python_wrappers_check_their_tensors():
                    dict(q_norm=torch.ones(32)), dict(q_out=torch.zeros(3, 4, 64).half()), dict()):
         with pytest.raises(rf.FoxError):
             rf.qk_norm_rope(**{**dict(x=rows, n_head=4, n_head_kv=2, head_dim=64, pos=pos, cos=cos, sin=cos), **change})
+
+
+def test_the_struct_is_laid_out_as_the_header_says(tmp_path):
+    import pathlib
+    import subprocess
+
+    import rustfox_b200.api as api
+    names = [f[0] for f in api.Kv4._fields_]
+    src = tmp_path / "kv4.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "foxcuda.h"\nint main(void) {\n'
+                   + "".join(f'  printf("%zu\\n", offsetof(foxcuda_kv4, {n}));\n' for n in names)
+                   + '  printf("%zu\\n", sizeof(foxcuda_kv4));\n  return 0;\n}\n')
+    include = pathlib.Path(__file__).resolve().parent.parent / "include"
+    subprocess.run(["gcc", "-I", str(include), "-o", str(tmp_path / "kv4"), str(src)], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "kv4")], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [getattr(api.Kv4, n).offset for n in names] + [C.sizeof(api.Kv4)]
+
+
+def test_outputs_that_overlap_are_refused(buf):
+    """Other blocks of the launch may still read what one writes."""
+    rf, L = _lib()
+    c = _view(rf, buf)
+    rows = c.n_rows * c.n_head_kv * c.head_dim * 4
+    assert L.foxcuda_kv4_read(C.byref(c), 0, buf, buf + rows - 16, None) == 1
+    assert b"overlap" in L.foxcuda_last_error()
+    assert L.foxcuda_kv4_attention(C.byref(c), 0, buf, 256, 4, 0.0, buf, 1 << 40, buf, None) == 1
+    assert b"overlap" in L.foxcuda_last_error()

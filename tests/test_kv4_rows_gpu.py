@@ -203,3 +203,39 @@ def test_a_captured_call_follows_its_device_lengths():
         g.replay()
         want = R.attend(host(q.double()), c.data, c.table, starts(rows), lens, np.full((2 * T, heads, hd), -2.0))
         _close(host(out.double()), want, "f32", (rows, lens))
+
+
+@pytest.mark.parametrize("T", [1, 5])
+def test_single_tokens_and_a_group_of_v_that_is_not_a_number(T):
+    """The other kernel (few rows): NaN in one group of V stays in its 64
+    dimensions there too."""
+    heads, kv, hd, L = 8, 2, 128, 150
+    c = Cache([L], kv, hd, seed=16)
+    q = _q(c, T, heads, hd)
+    want = R.attend(host(q.double()), c.data, c.table, [0, T], [L], np.zeros((T, heads, hd)))
+    o = R.PAGE * hd // 2 + 70 % R.PAGE * 8 + 4
+    c.data[c.table[0, 1], :, 1, o:o + 4] = 0xFF
+    got = _attend(c, q, [T], [L])
+    assert np.isnan(got[..., 64:]).all()
+    _close(np.ascontiguousarray(got[..., :64]), np.ascontiguousarray(want[..., :64]), "f32")
+
+
+def test_calls_on_two_streams_with_their_own_workspaces():
+    heads, kv, hd, T = 16, 4, 128, 16
+    c = Cache([5000, 3500], kv, hd, seed=17)
+    cache, table = c.on_device()
+    q = _q(c, 2 * T, heads, hd)
+    rs, kl = i32([0, T, 2 * T]), i32([5000, 3500])
+    want = rf.kv4_attention(q, cache, table, rs, kl)
+    one = rf.kv4_attention(q[:1], cache, table[:1].contiguous(), i32([0, 1]), i32([5000]))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(40):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(rf.kv4_attention(q, cache, table, rs, kl) if i % 4 < 2 else
+                        rf.kv4_attention(q[:1], cache, table[:1].contiguous(), i32([0, 1]), i32([5000])))
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, want if i % 4 < 2 else one), i
+    rf.kernel_errors()
