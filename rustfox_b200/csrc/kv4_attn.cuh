@@ -29,6 +29,15 @@
 //   from it. What cancels in the end must not pass through them: with all
 //   positions counted from below the error was 1e-4 of the result at 32768
 //   positions, now it is 1e-6.
+//
+// Bound by memory for long single tokens, with the issue of instructions close
+// behind: 16 sequences of 32768 positions, 32 heads over 8 of 128, take 122 us,
+// 4.9 TB/s of codes and parameters; 64 ragged fp16 ones over 16 KV heads 129 us,
+// 4.7 TB/s. Short ones are bound by their chain of dependent loads (row, length,
+// page, codes) and the launch: 576 positions 11 us, 65 positions 8 us. With many
+// rows the products and the weights of every row bound it: 32 (row, head) pairs
+// for each of 8 KV heads, 4 sequences of 8192 positions, 71 us; from 48 pairs on
+// the tiles of kv4_wide.cuh are faster.
 #pragma once
 
 #include <climits>
@@ -768,7 +777,8 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
   }
 }
 
-// Joins the CTAs' pieces of split runs, in the line's order. A pair of a run
+// Joins the CTAs' pieces of split runs, in the line's order: at most two pieces
+// a CTA, so its time is its launch's, part of which overlaps the first kernel. A pair of a run
 // takes 1, 2, 4 or 8 of the CTA's warps, by how many pieces a run has on
 // average; each takes every such-th piece.
 constexpr int KV4_JOIN_WARPS = 8;
