@@ -26,15 +26,17 @@
 //   The reference point of a pair's weights moves only when a score passes it
 //   by 2^KV4_SLACK; then, and every KV4_WIDE_FLUSH pages, O leaves tensor
 //   memory for the threads' registers, which bounds what the products' rounding
-//   toward zero adds up to.
+//   toward zero adds up to: 1.3e-6 of the result at every 4 pages, 2.1e-6 and
+//   0.6 % of the time less at every 8.
 // The work is divided as in kv4_attn.cuh, with a CTA for a warp.
 //
-// 64 rows behind 16384 positions, 32 heads over 8 of 128, take 84 us: 203
+// 64 rows behind 16384 positions, 32 heads over 8 of 128, take 84 us: 205
 // TFLOP/s of the formula's products, of which this form issues three for one and
-// the offsets. A page takes a tile about 4500 cycles, the products 1700 of them;
-// the unpacking warps' 20 instructions a word of codes and the weights' 12 an
-// element share the schedulers with them, and that is what bounds it. The time
-// hardly depends on how many of the 128 pairs are live.
+// the offsets. A page takes a tile about 4300 cycles, and K's three warps are
+// what it waits for (1200 cycles for the parameters and their exchange, 1800 for
+// the codes); the products take 1700, the weights 2000. With four warps for K
+// and three for V, V's are waited for instead, in the same time. The time hardly
+// depends on how many of the 128 pairs are live.
 #pragma once
 
 #include "kv4_attn.cuh"
@@ -144,6 +146,24 @@ FOX_DEV bool kv4_elect() {
   uint32_t r;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
   return r != 0;
+}
+
+// Two floats in one register pair: one instruction for both.
+typedef unsigned long long f32x2;
+FOX_DEV f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+FOX_DEV float2 unpack2(f32x2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+FOX_DEV f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // 8 codes as fp16 2 c - 15, in the order (0, 4), (1, 5), (2, 6), (3, 7).
@@ -401,15 +421,19 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         const float base = 7.0f - (mx == -INFINITY ? 0.0f : mx);
         static_assert(KV4_SLACK == 7.0f, "2^14, and not fp16's 2^16");
         uint32_t hi[A::POS / 2], lo[A::POS / 2];
+        f32x2 l2 = 0;
 #pragma unroll
         for (int i = 0; i < A::POS; i += 2) {
+          // (a packed product and sum were fused by the assembler; these are not)
           const float w0 = exp2_approx(__fadd_rn(__fmul_rn(__uint_as_float(d[i]), fj), base));
           const float w1 = exp2_approx(__fadd_rn(__fmul_rn(__uint_as_float(d[i + 1]), fj), base));
-          l += w0 + w1;
+          l2 = add2(l2, pack2(w0, w1));
           const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
+          const float2 r = unpack2(add2(pack2(w0, w1), pack2(-h0, -h1)));
           hi[i / 2] = half2_bits(__floats2half2_rn(h0, h1));
-          lo[i / 2] = half2_bits(__floats2half2_rn(w0 - h0, w1 - h1));
+          lo[i / 2] = half2_bits(__floats2half2_rn(r.x, r.y));
         }
+        l += unpack2(l2).x + unpack2(l2).y;
 #pragma unroll
         for (int c = 0; c < A::POS / 2; c += 8) {
           const uint32_t(&h)[8] = *reinterpret_cast<const uint32_t(*)[8]>(hi + c);
