@@ -239,3 +239,28 @@ def test_calls_on_two_streams_with_their_own_workspaces():
     for i, o in enumerate(outs):
         assert torch.equal(o, want if i % 4 < 2 else one), i
     rf.kernel_errors()
+
+
+def test_as_many_sequences_as_a_call_takes():
+    """1024 ragged sequences of 12 rows of 4 heads that share a prefix's pages,
+    some of them empty; then all of them."""
+    heads, kv, hd, n, T = 4, 1, 128, 1024, 12
+    c = Cache([256], kv, hd, seed=18)
+    table = np.full((n, WIDE), -1, np.int32)
+    table[:, :4] = c.table
+    lens = c.rng.integers(0, 257, n)
+    rs = np.arange(n + 1) * T
+    q = _q(c, n * T, heads, hd)
+    args = dev(c.data), dev(table), i32(rs)
+    got = host(rf.kv4_attention(q, *args, i32(lens)).double())
+    for s in range(0, n, 37):
+        a, b = rs[s], rs[s + 1]
+        want = R.attend(host(q[a:b].double()), c.data, table[s:s + 1], [0, T], lens[s:s + 1], np.zeros((T, heads, hd)))
+        if lens[s]:
+            _close(got[a:b], want, "f32", (s, lens[s]))
+        else:
+            assert (got[a:b] == 0).all()
+    out = torch.full_like(q, 3.0)
+    rf.kv4_attention(q, *args, i32([0] * n), out=out)
+    assert (out == 0).all()
+    rf.kernel_errors()
