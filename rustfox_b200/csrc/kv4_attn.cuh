@@ -777,8 +777,10 @@ __global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel
   }
 }
 
-// Joins the CTAs' pieces of split runs, in the line's order: at most two pieces
-// a CTA, so its time is its launch's, part of which overlaps the first kernel. A pair of a run
+// Joins the CTAs' pieces of split runs, in the line's order. Bound by the
+// blocks' way to their pieces, not by the bytes: alone and cold 10 us for the
+// 128 runs of 16 sequences (0.6 MB from memory), 16 us for the 16 runs of 128
+// pairs of 64 rows (11 MB); in a call its start overlaps the first kernel's end. A pair of a run
 // takes 1, 2, 4 or 8 of the CTA's warps, by how many pieces a run has on
 // average; each takes every such-th piece.
 constexpr int KV4_JOIN_WARPS = 8;
