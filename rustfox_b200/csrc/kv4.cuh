@@ -36,7 +36,9 @@ __host__ __device__ constexpr int kv4_block_bytes(int hd) { return KV_PAGE * (hd
 __host__ __device__ constexpr int kv4_codes_bytes(int hd) { return KV_PAGE * hd / 2; }
 
 // Rows of sequences: sequence s has the rows row_start[s] ..
-// row_start[s+1]-1, standing at the last of its kv_len[s] cached positions.
+// row_start[s+1]-1, standing at the last of its kv_len[s] positions. The length
+// as given places them, also where the block table holds fewer positions: rows
+// and positions outside it are absent, and move no others.
 struct Kv4Rows {
   uint8_t* cache;
   const int* table;      // [n_seq][table_stride] pages
@@ -46,12 +48,13 @@ struct Kv4Rows {
   int* err;
 };
 
-// Cached positions of sequence s, held to its block table (an overrun is
-// reported once per call of this).
-FOX_DEV int kv4_len(const Kv4Rows& c, int s) {
-  const int L = __ldg(c.kv_len + s), most = c.table_stride * KV_PAGE;
-  if (L > most && c.err) atomicExch(c.err, KERR_PAGES);
-  return min(max(L, 0), most);
+// The length of sequence s as given, and what of it its block table holds (less
+// is reported once per call of this).
+FOX_DEV int kv4_len(const Kv4Rows& c, int s) { return max(__ldg(c.kv_len + s), 0); }
+FOX_DEV int kv4_held(const Kv4Rows& c, int len) {
+  const int most = c.table_stride * KV_PAGE;
+  if (len > most && c.err) atomicExch(c.err, KERR_PAGES);
+  return min(len, most);
 }
 
 // The page of sequence s that holds position p (inside the table), or -1
@@ -63,7 +66,8 @@ FOX_DEV int kv4_page(const Kv4Rows& c, int s, int p) {
   return -1;
 }
 
-// A row's page and position in it; page -1 for rows that have none.
+// A row's page and position in it; page -1 for rows that have none (reported
+// where the row stands behind the table's end).
 struct Kv4Place { int page, at; };
 FOX_DEV Kv4Place kv4_place(const Kv4Rows& c, int row) {
   Kv4Place x = {-1, 0};
@@ -75,7 +79,7 @@ FOX_DEV Kv4Place kv4_place(const Kv4Rows& c, int row) {
   }
   if (lo >= c.n_seq) return x;
   const int pos = kv4_len(c, lo) - (__ldg(c.row_start + lo + 1) - row);
-  if (pos < 0) return x;
+  if (pos < 0 || kv4_held(c, pos + 1) <= pos) return x;
   x.page = kv4_page(c, lo, pos);
   x.at = pos % KV_PAGE;
   return x;

@@ -73,14 +73,18 @@ constexpr int KV4_WHOLE = 16;
 // A run begins with KV4_HEAD units without a page: what its queries' loading
 // and its results' writing take of a worker's time.
 constexpr int KV4_HEAD = 2;
-struct Kv4Seq { int r0, T, L, tiles, units; };
+// Rows r0 .. r0 + T - 1, the first at position at (negative: it has none), and
+// the L positions that the block table holds.
+struct Kv4Seq { int r0, T, at, L, tiles, units; };
 
 template <int PAIRS>
 FOX_DEV Kv4Seq kv4_seq(const Kv4AttnParams& p, int s) {
   Kv4Seq q;
   q.r0 = min(max(__ldg(p.c.row_start + s), 0), p.c.n_rows);
   q.T = min(max(__ldg(p.c.row_start + s + 1), q.r0), p.c.n_rows) - q.r0;
-  q.L = kv4_len(p.c, s);
+  const int len = kv4_len(p.c, s);
+  q.at = len - q.T;
+  q.L = kv4_held(p.c, len);
   q.tiles = (q.T * (p.n_head / p.c.n_kv) + PAIRS - 1) / PAIRS;
   q.units = KV4_HEAD + (q.L + KV_PAGE - 1) / KV_PAGE;
   return q;
@@ -291,7 +295,7 @@ struct Kv4Attn {
 
   // The last position that any row of a tile sees.
   static FOX_DEV int last_seen(const Kv4Seq& q, int tile, int gqa) {
-    return q.L - q.T + min(q.T - 1, (tile * PAIRS + PAIRS - 1) / gqa);
+    return q.at + min(q.T - 1, (tile * PAIRS + PAIRS - 1) / gqa);
   }
 
   template <typename T>
@@ -300,9 +304,9 @@ struct Kv4Attn {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int pr = it.tile * PAIRS + n * 4 + t;
-      lim[n] = pr < it.q.T * gqa ? it.q.L - it.q.T + pr / gqa : INT_MAX;
+      lim[n] = pr < it.q.T * gqa ? it.q.at + pr / gqa : INT_MAX;
     }
-    lim_min = max(0, it.q.L - it.q.T + it.tile * PAIRS / gqa);
+    lim_min = max(0, it.q.at + it.tile * PAIRS / gqa);
     lim_max = last_seen(it.q, it.tile, gqa);
     const float unit = p.scale * 1.44269504088896341f;
 #pragma unroll

@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
     r.next = min(run_end, a1);
     r.begins = in_run == 0;
     r.ends = r.next == run_end;
-    r.lim_max = r.x.q.L - r.x.q.T + min(r.x.q.T - 1, (r.x.tile * PAIRS + PAIRS - 1) / gqa);
+    r.lim_max = r.x.q.at + min(r.x.q.T - 1, (r.x.tile * PAIRS + PAIRS - 1) / gqa);
     r.first = max(r.x.page, 0);
     r.last = max(r.first, min(r.x.page + (r.next - u), r.lim_max < 0 ? 0 : r.lim_max / KV_PAGE + 1));
     return r;
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
       const int pr = r.x.tile * PAIRS + pair;
       const bool live = pr < r.x.q.T * gqa;
       const int row = live ? pr / gqa : 0, head = r.x.kv * gqa + (live ? pr - row * gqa : 0);
-      const int lim = live ? r.x.q.L - r.x.q.T + row : INT_MAX, lim_min = max(0, r.x.q.L - r.x.q.T + r.x.tile * PAIRS / gqa);
+      const int lim = live ? r.x.q.at + row : INT_MAX, lim_min = max(0, r.x.q.at + r.x.tile * PAIRS / gqa);
       float f = 0.0f;
       // q's operand: this thread's OWN dimensions of its pair
       if (r.last > r.first) {
