@@ -196,10 +196,10 @@ foxcuda_status foxcuda_attention(const float *q, const void *kcache, const void 
  *   Entries behind a sequence's last page are not read. Sequences may share
  *   pages that no row of the call is written to.
  * - What the device arrays place outside their bounds (a page outside the
- *   cache, a position behind table_stride pages) is skipped, the position as if
- *   it were absent, and reported by foxcuda_kernel_errors; the other rows and
- *   positions stay where they are. row_start must not fall; it is held to
- *   n_rows.
+ *   cache, a position behind table_stride pages, a row from n_rows on) is
+ *   skipped, the position as if it were absent, and reported by
+ *   foxcuda_kernel_errors; the other rows and positions stay where they are.
+ *   row_start must not fall.
  * - head_dim 64, 128 or 256; at most 1024 sequences and 2^20 rows; the cache
  *   and the row arrays 16-byte aligned, row strides (in elements) a multiple
  *   of 16 bytes. No call allocates or synchronises, and each can be captured;

@@ -36,9 +36,9 @@ __host__ __device__ constexpr int kv4_block_bytes(int hd) { return KV_PAGE * (hd
 __host__ __device__ constexpr int kv4_codes_bytes(int hd) { return KV_PAGE * hd / 2; }
 
 // Rows of sequences: sequence s has the rows row_start[s] ..
-// row_start[s+1]-1, standing at the last of its kv_len[s] positions. The length
-// as given places them, also where the block table holds fewer positions: rows
-// and positions outside it are absent, and move no others.
+// row_start[s+1]-1, standing at the last of its kv_len[s] positions. Both as
+// given place them, also where the block table holds fewer positions or the row
+// arrays fewer rows: what lies outside is absent, and moves nothing else.
 struct Kv4Rows {
   uint8_t* cache;
   const int* table;      // [n_seq][table_stride] pages
@@ -67,10 +67,12 @@ FOX_DEV int kv4_page(const Kv4Rows& c, int s, int p) {
 }
 
 // A row's page and position in it; page -1 for rows that have none (reported
-// where the row stands behind the table's end).
+// where the row stands behind the table's end). The last row reports rows that
+// are not there.
 struct Kv4Place { int page, at; };
 FOX_DEV Kv4Place kv4_place(const Kv4Rows& c, int row) {
   Kv4Place x = {-1, 0};
+  if (row == c.n_rows - 1 && __ldg(c.row_start + c.n_seq) > c.n_rows && c.err) atomicExch(c.err, KERR_PAGES);
   if (row >= c.n_rows || row < __ldg(c.row_start)) return x;
   int lo = 0, hi = c.n_seq;  // sequences that end at or before the row
   while (lo < hi) {

@@ -81,9 +81,10 @@ template <int PAIRS>
 FOX_DEV Kv4Seq kv4_seq(const Kv4AttnParams& p, int s) {
   Kv4Seq q;
   q.r0 = min(max(__ldg(p.c.row_start + s), 0), p.c.n_rows);
-  q.T = min(max(__ldg(p.c.row_start + s + 1), q.r0), p.c.n_rows) - q.r0;
-  const int len = kv4_len(p.c, s);
-  q.at = len - q.T;
+  const int end = max(__ldg(p.c.row_start + s + 1), q.r0), len = kv4_len(p.c, s);
+  if (end > p.c.n_rows && p.c.err) atomicExch(p.c.err, KERR_PAGES);
+  q.T = min(end, p.c.n_rows) - q.r0;
+  q.at = len - (end - q.r0);
   q.L = kv4_held(p.c, len);
   q.tiles = (q.T * (p.n_head / p.c.n_kv) + PAIRS - 1) / PAIRS;
   q.units = KV4_HEAD + (q.L + KV_PAGE - 1) / KV_PAGE;
