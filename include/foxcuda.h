@@ -199,7 +199,8 @@ foxcuda_status foxcuda_attention(const float *q, const void *kcache, const void 
  *   cache, a position behind table_stride pages, a row from n_rows on) is
  *   skipped, the position as if it were absent, and reported by
  *   foxcuda_kernel_errors; the other rows and positions stay where they are.
- *   row_start must not fall.
+ *   row_start must not fall: attention reports one that does, and leaves all
+ *   rows as they were.
  * - head_dim 64, 128 or 256; at most 1024 sequences and 2^20 rows; the cache
  *   and the row arrays 16-byte aligned, row strides (in elements) a multiple
  *   of 16 bytes. No call allocates or synchronises, and each can be captured;

@@ -111,7 +111,8 @@ struct Kv4Line {
   bool whole;  // no run is split between CTAs
   static __host__ __device__ int bytes(int n_seq) { return (2 * n_seq + 3) * 4; }
 
-  // By the CTA's first warp; every thread calls.
+  // By the CTA's first warp; every thread calls. A row_start that falls could
+  // count rows twice and the units past 2^31: it leaves the line empty.
   template <int PAIRS>
   FOX_DEV void build(const Kv4AttnParams& p, void* mem) {
     n_seq = p.c.n_seq;
@@ -120,11 +121,13 @@ struct Kv4Line {
     const int lane = threadIdx.x & 31;
     if (threadIdx.x < 32) {
       int r0 = 0, u0 = 0, longest = 0;
+      bool falls = false;
       for (int s0 = 0; s0 < n_seq; s0 += 32) {
         const int s = s0 + lane;
         int r = 0, n = 0;
         if (s < n_seq) {
           const Kv4Seq q = kv4_seq<PAIRS>(p, s);
+          falls = falls || __ldg(p.c.row_start + s + 1) < __ldg(p.c.row_start + s);
           r = q.tiles * p.c.n_kv;
           n = r * q.units;
           if (r) longest = max(longest, q.units);
@@ -138,6 +141,11 @@ struct Kv4Line {
         if (s < n_seq) { run0[s] = r0 + rs - r; unit0[s] = u0 + ns - n; }
         r0 += __shfl_sync(0xffffffffu, rs, 31);
         u0 += __shfl_sync(0xffffffffu, ns, 31);
+        if (__any_sync(0xffffffffu, falls)) {
+          if (lane == 0 && p.c.err) atomicExch(p.c.err, KERR_PAGES);
+          r0 = u0 = 0;
+          break;
+        }
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
