@@ -168,7 +168,7 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
   RopeParams p{};
   p.x = x; p.pos = pos; p.q_norm = q_norm; p.k_norm = k_norm; p.cos = cos; p.sin = sin; p.q = q_out; p.k = k_out;
   p.x_stride = x_stride; p.q_stride = q_stride; p.k_stride = k_stride;
-  p.n_rows = (int)n_rows; p.n_head = (int)n_head; p.n_kv = (int)n_head_kv; p.n_pos = (int)n_pos; p.halves = halves;
+  p.n_rows = (int)n_rows; p.n_head = (int)n_head; p.n_kv = (int)n_head_kv; p.n_pos = (int)n_pos;
   p.eps = eps; p.err = kernel_err_ptr();
   CK(by_type_hd(type, head_dim, [&](auto tag, auto hd) {
        return halves ? launch_rope<decltype(tag), hd.value, true>(p, (cudaStream_t)stream)
@@ -181,7 +181,7 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
 template <int HD>
 static size_t kv4_work_bytes(int ctas) {
   constexpr int wide = HD < 256 ? KV4_WIDE_PAIRS : 0;
-  return (size_t)ctas * 2 * std::max(wide, Kv4Attn<HD, 1>::PAIRS) * (HD + 4) * 4;
+  return (size_t)ctas * 2 * std::max(wide, Kv4Attn<HD>::PAIRS) * (HD + 4) * 4;
 }
 
 extern "C" size_t foxcuda_kv4_attention_workspace(uint32_t head_dim, uint32_t table_stride) {
@@ -230,10 +230,10 @@ static cudaError_t launch_kv4_attend(const Kv4AttnParams& p, bool wide, cudaStre
       return launch_kv4_join<T, HD, A::PAIRS>(p, s);
     }
   }
-  using A = Kv4Attn<HD, 1>;
+  using A = Kv4Attn<HD>;
   const size_t smem = A::smem_bytes(p.c.n_seq);
-  if ((e = opt_in_smem(kv4_attend_kernel<HD, T, 1>, smem, marks[0])) != cudaSuccess) return e;
-  kv4_attend_kernel<HD, T, 1><<<p.ctas, A::NW * 32, smem, s>>>(p);
+  if ((e = opt_in_smem(kv4_attend_kernel<HD, T>, smem, marks[0])) != cudaSuccess) return e;
+  kv4_attend_kernel<HD, T><<<p.ctas, A::NW * 32, smem, s>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess || !join) return e;
   return launch_kv4_join<T, HD, A::PAIRS>(p, s);
 }

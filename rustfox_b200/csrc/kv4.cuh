@@ -387,7 +387,7 @@ struct RopeParams {
   const float *cos, *sin;        // [n_pos][hd / 2]
   void *q, *k;
   size_t x_stride, q_stride, k_stride;
-  int n_rows, n_head, n_kv, n_pos, halves;
+  int n_rows, n_head, n_kv, n_pos;
   float eps;
   int* err;
 };
@@ -426,7 +426,7 @@ FOX_DEV void rope_store(__half* p, const float (&v)[8]) { kv4_store8(p, v); }
 // RMSNorm of every query and key head and the rotation of its position:
 //   y = x * (1 / sqrt(mean(x^2) + eps)) * w
 //   (a, b) -> (a cos - b sin, a sin + b cos) for the pairs (2i, 2i+1), or
-//   (i, i + hd/2) when halves is set.
+//   (i, i + hd/2) with HALVES.
 // A lane holds E neighbouring dimensions of a head (16 bytes, or 32 of 256
 // fp32 dimensions), so the pairs lie in a lane and the halves LANES / 2 lanes
 // apart. A warp takes BATCH such loads of one row's query or key heads, so that

@@ -270,13 +270,13 @@ struct Kv4Sum {
   }
 };
 
-// HD: head dimension; NT: column tiles (of 4 pairs) of a warp.
-template <int HD, int NT>
+// HD: head dimension.
+template <int HD>
 struct Kv4Attn {
   static constexpr int SLAB = HD < 128 ? HD : 128, SLABS = HD / SLAB, SG = SLAB / 64, NB = SLAB / 32;
   static constexpr int G = HD / KV4_GROUP, BB = kv4_block_bytes(HD), PAGE_BYTES = 2 * BB;
-  static constexpr int PAIRS = 4 * NT;       // (row, head) pairs of a tile
-  static constexpr int SUM_VECS = NT * SLABS * NB * 2;  // float4s of a lane's sums
+  static constexpr int PAIRS = 4;            // (row, head) pairs of a tile
+  static constexpr int SUM_VECS = SLABS * NB * 2;  // float4s of a lane's sums
   static constexpr int PART = HD + 4;        // floats of one pair's partial result: M, l, -, -, sums
   // warps of a CTA: what the registers (and for 256 dimensions shared memory)
   // hold. Each has room for a page's K and V, then for a piece of a run; for
@@ -289,18 +289,18 @@ struct Kv4Attn {
 
   // A warp's share of a tile: q's operand registers, and the running maximum,
   // weights and sums of its pairs. Lane (g, t) = (lane / 4, lane % 4) holds
-  // the scores of pair t of each column tile at positions g and g + 8 of a
-  // step, and the sums of dimensions 4g .. 4g+3 of each block of 32.
-  uint32_t qb[NT][SLABS][SG][2][2][2];
-  float f[NT], qs[NT][G];  // score = f * sum_g (d_g * product) + sum_g m_g * qs_g, in powers of 2
-  float o[NT][SLABS][NB][2][4], mx[NT], l[NT], mo[NT][G], big;
+  // the scores of pair t at positions g and g + 8 of a step, and pair t's sums of
+  // dimensions 4g .. 4g+3 of each block of 32.
+  uint32_t qb[SLABS][SG][2][2][2];
+  float f, qs[G];  // score = f * sum_g (d_g * product) + sum_g m_g * qs_g, in powers of 2
+  float o[SLABS][NB][2][4], mx, l, mo[G], big;
   // The matrix instructions round their sums toward zero, 0.7 * 2^-24 of them
   // each time, so after KV4_FLUSH pages they move to shared memory (this
   // lane's float4s, 32 apart), added to the nearest. `flushed`: there are any.
   float4* sums;
   bool flushed;
-  float sco[NT][4][2];            // the page's scores
-  int lim[NT], lim_min, lim_max;  // the last position a pair sees (negative: none; no pair: all), and over the tile
+  float sco[4][2];            // the page's scores
+  int lim, lim_min, lim_max;  // the last position pair t sees (negative: none; no pair: all), and over the tile
 
   // The last position that any row of a tile sees.
   static FOX_DEV int last_seen(const Kv4Seq& q, int tile, int gqa) {
@@ -310,99 +310,90 @@ struct Kv4Attn {
   template <typename T>
   FOX_DEV void begin(const Kv4AttnParams& p, const Kv4Unit& it, int gqa) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int pr = it.tile * PAIRS + n * 4 + t;
-      lim[n] = pr < it.q.T * gqa ? it.q.at + pr / gqa : INT_MAX;
-    }
+    lim = it.tile * PAIRS + t < it.q.T * gqa ? it.q.at + (it.tile * PAIRS + t) / gqa : INT_MAX;
     lim_min = max(0, it.q.at + it.tile * PAIRS / gqa);
     lim_max = last_seen(it.q, it.tile, gqa);
     const float unit = p.scale * 1.44269504088896341f;
+    const int pr = it.tile * PAIRS + (g >> 1);
+    const bool live = pr < it.q.T * gqa;
+    const int row = it.q.r0 + (live ? pr / gqa : 0), head = it.kv * gqa + (live ? pr % gqa : 0);
+    const T* q = static_cast<const T*>(p.q) + (size_t)row * p.q_stride + (size_t)head * HD;
+    float x[G][16], top = 0.0f, sum[G];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int pr = it.tile * PAIRS + n * 4 + (g >> 1);
-      const bool live = pr < it.q.T * gqa;
-      const int row = it.q.r0 + (live ? pr / gqa : 0), head = it.kv * gqa + (live ? pr % gqa : 0);
-      const T* q = static_cast<const T*>(p.q) + (size_t)row * p.q_stride + (size_t)head * HD;
-      float x[G][16], top = 0.0f, sum[G];
+    for (int j = 0; j < G; ++j) {
+      sum[j] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        sum[j] = 0.0f;
+      for (int i = 0; i < 4; ++i) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (live) v = kv4_load4(q + j * 64 + t * 16 + i * 4);
+        x[j][4 * i] = v.x; x[j][4 * i + 1] = v.y; x[j][4 * i + 2] = v.z; x[j][4 * i + 3] = v.w;
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (live) v = kv4_load4(q + j * 64 + t * 16 + i * 4);
-          x[j][4 * i] = v.x; x[j][4 * i + 1] = v.y; x[j][4 * i + 2] = v.z; x[j][4 * i + 3] = v.w;
+      for (int i = 0; i < 16; ++i) { sum[j] += x[j][i]; top = fmaxf(top, fabsf(x[j][i])); }
+      sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
+      sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // the power of two that takes the largest |q| to [2^13, 2^14)
+    const int e = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -100), 100);
+    const float sc = __uint_as_float((uint32_t)(e + 127) << 23);
+    const float back = unit * KV4_EVEN * __uint_as_float((uint32_t)(127 - e) << 23);
+    f = __shfl_sync(0xffffffffu, back, t * 8);
+#pragma unroll
+    for (int j = 0; j < G; ++j) qs[j] = __shfl_sync(0xffffffffu, sum[j], t * 8) * unit;
+    auto part = [&](float v, float by) {
+      v *= sc * by;
+      const float hi = __uint_as_float(__float_as_uint(v) & 0xffffe000u);
+      return g & 1 ? v - hi : hi;
+    };
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float* v = &x[j][8 * w + 2 * h];
+          uint32_t* b = qb[j / SG][j % SG][w][h];
+          b[0] = half2_bits(__floats2half2_rn(part(v[0], 1.0f), part(v[4], 1.0f)));
+          b[1] = half2_bits(__floats2half2_rn(part(v[1], 0.0625f), part(v[5], 0.0625f)));
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { sum[j] += x[j][i]; top = fmaxf(top, fabsf(x[j][i])); }
-        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
-        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // the power of two that takes the largest |q| to [2^13, 2^14)
-      const int e = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -100), 100);
-      const float sc = __uint_as_float((uint32_t)(e + 127) << 23);
-      const float back = unit * KV4_EVEN * __uint_as_float((uint32_t)(127 - e) << 23);
-      f[n] = __shfl_sync(0xffffffffu, back, t * 8);
+    for (int sl = 0; sl < SLABS; ++sl)
 #pragma unroll
-      for (int j = 0; j < G; ++j) qs[n][j] = __shfl_sync(0xffffffffu, sum[j], t * 8) * unit;
-      auto part = [&](float v, float by) {
-        v *= sc * by;
-        const float hi = __uint_as_float(__float_as_uint(v) & 0xffffe000u);
-        return g & 1 ? v - hi : hi;
-      };
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int j = 0; j < G; ++j)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+          for (int c = 0; c < 4; ++c) o[sl][b][h][c] = 0.0f;
+    mx = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float* v = &x[j][8 * w + 2 * h];
-            uint32_t* b = qb[n][j / SG][j % SG][w][h];
-            b[0] = half2_bits(__floats2half2_rn(part(v[0], 1.0f), part(v[4], 1.0f)));
-            b[1] = half2_bits(__floats2half2_rn(part(v[1], 0.0625f), part(v[5], 0.0625f)));
-          }
-#pragma unroll
-      for (int sl = 0; sl < SLABS; ++sl)
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[n][sl][b][h][c] = 0.0f;
-      mx[n] = -INFINITY;
-      l[n] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < G; ++j) mo[n][j] = 0.0f;
-    }
+    for (int j = 0; j < G; ++j) mo[j] = 0.0f;
     big = 0x1p-24f;  // a power of two above every d met
     flushed = false;
   }
 
-  FOX_DEV float4 sum_of(int n, int sl, int b, int h) const {
-    const float(&c)[4] = o[n][sl][b][h];
+  FOX_DEV float4 sum_of(int sl, int b, int h) const {
+    const float(&c)[4] = o[sl][b][h];
     float4 v = make_float4(c[0], c[1], c[2], c[3]);
     if (flushed) {
-      const float4 w = sums[32 * (((n * SLABS + sl) * NB + b) * 2 + h)];
+      const float4 w = sums[32 * ((sl * NB + b) * 2 + h)];
       v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
     }
     return v;
   }
   FOX_DEV void flush() {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int sl = 0; sl < SLABS; ++sl)
 #pragma unroll
-      for (int sl = 0; sl < SLABS; ++sl)
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int h = 0; h < 2; ++h) {
+          sums[32 * ((sl * NB + b) * 2 + h)] = sum_of(sl, b, h);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            sums[32 * (((n * SLABS + sl) * NB + b) * 2 + h)] = sum_of(n, sl, b, h);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[n][sl][b][h][c] = 0.0f;
-          }
+          for (int c = 0; c < 4; ++c) o[sl][b][h][c] = 0.0f;
+        }
     flushed = true;
   }
 
@@ -413,7 +404,7 @@ struct Kv4Attn {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int a = s * 16 + g;
-      float prod[NT][2], off[NT][2];
+      float prod[2], off[2];
 #pragma unroll
       for (int sl = 0; sl < SLABS; ++sl) {
         uint32_t wa[2 * SG], wb[2 * SG];
@@ -428,35 +419,27 @@ struct Kv4Attn {
 #pragma unroll
         for (int j = 0; j < SG; ++j) {
           const int gg = sl * SG + j;
-          float c[NT][4];
+          float c[4];
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             uint32_t x[4], y[4];
             kv4_operands(wa[2 * j + w], x);
             kv4_operands(wb[2 * j + w], y);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const uint32_t(&b)[2][2] = qb[n][sl][j][w];
-              if (w == 0) mma16816_0(c[n], x[0], y[0], x[1], y[1], b[0][0], b[0][1]);
-              else mma16816(c[n], x[0], y[0], x[1], y[1], b[0][0], b[0][1]);
-              mma16816(c[n], x[2], y[2], x[3], y[3], b[1][0], b[1][1]);
-            }
+            const uint32_t(&b)[2][2] = qb[sl][j][w];
+            if (w == 0) mma16816_0(c, x[0], y[0], x[1], y[1], b[0][0], b[0][1]);
+            else mma16816(c, x[0], y[0], x[1], y[1], b[0][0], b[0][1]);
+            mma16816(c, x[2], y[2], x[3], y[3], b[1][0], b[1][1]);
           }
           const float2 da = __half22float2(dm[a * G + gg]), db = __half22float2(dm[(a + 8) * G + gg]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float ca = c[n][0] + c[n][1], cb = c[n][2] + c[n][3];
-            prod[n][0] = gg ? fmaf(da.x, ca, prod[n][0]) : da.x * ca;
-            prod[n][1] = gg ? fmaf(db.x, cb, prod[n][1]) : db.x * cb;
-            off[n][0] = gg ? fmaf(da.y, qs[n][gg], off[n][0]) : da.y * qs[n][gg];
-            off[n][1] = gg ? fmaf(db.y, qs[n][gg], off[n][1]) : db.y * qs[n][gg];
-          }
+          const float ca = c[0] + c[1], cb = c[2] + c[3];
+          prod[0] = gg ? fmaf(da.x, ca, prod[0]) : da.x * ca;
+          prod[1] = gg ? fmaf(db.x, cb, prod[1]) : db.x * cb;
+          off[0] = gg ? fmaf(da.y, qs[gg], off[0]) : da.y * qs[gg];
+          off[1] = gg ? fmaf(db.y, qs[gg], off[1]) : db.y * qs[gg];
         }
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) sco[n][s][h] = fmaf(prod[n][h], f[n], off[n][h]);
+      for (int h = 0; h < 2; ++h) sco[s][h] = fmaf(prod[h], f, off[h]);
     }
   }
 
@@ -466,9 +449,9 @@ struct Kv4Attn {
   FOX_DEV void values(const uint8_t* vb, int pos0) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const __half2* dm = reinterpret_cast<const __half2*>(vb + kv4_codes_bytes(HD));
-    // this lane's parameters, the page's largest d, the maxima over its positions
+    // this lane's parameters, the page's largest d, the maximum over its positions
     __half2 dv[4][2][G], most = __half2half2(__ushort_as_half(0));
-    float top[NT];
+    float top;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -481,51 +464,41 @@ struct Kv4Attn {
           if (nobody) dv[s][h][j] = __half2half2(__ushort_as_half(0));  // whatever the memory held
           most = __hmax2(most, dv[s][h][j]);
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (EDGE && pos0 + at > lim[n]) sco[n][s][h] = -INFINITY;
-          top[n] = s + h ? fmaxf(top[n], sco[n][s][h]) : sco[n][s][h];
-        }
+        if (EDGE && pos0 + at > lim) sco[s][h] = -INFINITY;
+        top = s + h ? fmaxf(top, sco[s][h]) : sco[s][h];
       }
 #pragma unroll
     for (int sh = 4; sh < 32; sh <<= 1) {
       most = __hmax2(most, __shfl_xor_sync(0xffffffffu, most, sh));
-#pragma unroll
-      for (int n = 0; n < NT; ++n) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], sh));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
     }
     const float dmax = __low2float(most);
     // The reference point of a pair's weights moves only when a score passes
     // it by 2^KV4_SLACK: the weights' scale leaves room for that.
-    bool grew = dmax >= big;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) grew = grew || top[n] > mx[n] + KV4_SLACK;
-    if (__any_sync(0xffffffffu, grew)) {
+    if (__any_sync(0xffffffffu, dmax >= big || top > mx + KV4_SLACK)) {
       const float to = dmax >= big ? __uint_as_float((__float_as_uint(dmax) & 0x7f800000u) + 0x00800000u) : big;
       const float shrink = big / to;
       big = to;
+      const float m = fmaxf(mx, top);
+      const float al = m == -INFINITY ? 1.0f : exp2_approx(mx - m), all = al * shrink;
+      mx = m;
+      l *= al;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float m = fmaxf(mx[n], top[n]);
-        const float al = m == -INFINITY ? 1.0f : exp2_approx(mx[n] - m), all = al * shrink;
-        mx[n] = m;
-        l[n] *= al;
+      for (int j = 0; j < G; ++j) mo[j] *= al;
 #pragma unroll
-        for (int j = 0; j < G; ++j) mo[n][j] *= al;
+      for (int sl = 0; sl < SLABS; ++sl)
 #pragma unroll
-        for (int sl = 0; sl < SLABS; ++sl)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int b = 0; b < NB; ++b)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int c = 0; c < 4; ++c) o[sl][b][h][c] *= all;
+      if (flushed)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) o[n][sl][b][h][c] *= all;
-        if (flushed)
-#pragma unroll
-          for (int i = 0; i < SUM_VECS / NT; ++i) {
-            float4& v = sums[32 * (n * (SUM_VECS / NT) + i)];
-            v = make_float4(v.x * all, v.y * all, v.z * all, v.w * all);
-          }
-      }
+        for (int i = 0; i < SUM_VECS; ++i) {
+          float4& v = sums[32 * i];
+          v = make_float4(v.x * all, v.y * all, v.z * all, v.w * all);
+        }
     }
 
     // the weights, times d, as the second product's operand
@@ -537,27 +510,19 @@ struct Kv4Attn {
     for (int i = 0; i < 4; ++i) asm volatile("" : "+r"(flip[i / 2][i % 2]));  // held in registers
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      uint32_t pb[NT][G][2];
+      uint32_t pb[G][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const bool swap = (s + h) & 1;
-        float w[NT], wn[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          w[n] = exp2_approx(sco[n][s][h] - (EDGE && mx[n] == -INFINITY ? 0.0f : mx[n]));
-          wn[n] = w[n] * (swap ? -norm : norm);
-          l[n] += w[n];
-        }
+        const float w = exp2_approx(sco[s][h] - (EDGE && mx == -INFINITY ? 0.0f : mx)), wn = w * (swap ? -norm : norm);
+        l += w;
 #pragma unroll
         for (int j = 0; j < G; ++j) {
           const float2 d = __half22float2(dv[s][h][j]);
           const float m = fmaf(swap ? 15.0f - from_top : from_top, d.x, d.y);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const bool hidden = EDGE && sco[n][s][h] == -INFINITY;  // whatever it is
-            mo[n][j] = fmaf(w[n], hidden ? 0.0f : m, mo[n][j]);
-            pb[n][j][h] = transpose8x8(kv4_hi_lo(hidden ? 0.0f : wn[n] * d.x));
-          }
+          const bool hidden = EDGE && sco[s][h] == -INFINITY;  // whatever it is
+          mo[j] = fmaf(w, hidden ? 0.0f : m, mo[j]);
+          pb[j][h] = transpose8x8(kv4_hi_lo(hidden ? 0.0f : wn * d.x));
         }
       }
 #pragma unroll
@@ -577,11 +542,8 @@ struct Kv4Attn {
           uint32_t x[4], y[4];
           kv4_operands(u[b], flip[s & 1][0], flip[s & 1][1], x);
           kv4_operands(v[b], flip[1 - (s & 1)][0], flip[1 - (s & 1)][1], y);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma16816(o[n][sl][b][0], x[0], x[1], y[0], y[1], pb[n][j][0], pb[n][j][1]);
-            mma16816(o[n][sl][b][1], x[2], x[3], y[2], y[3], pb[n][j][0], pb[n][j][1]);
-          }
+          mma16816(o[sl][b][0], x[0], x[1], y[0], y[1], pb[j][0], pb[j][1]);
+          mma16816(o[sl][b][1], x[2], x[3], y[2], y[3], pb[j][0], pb[j][1]);
         }
       }
     }
@@ -594,37 +556,34 @@ struct Kv4Attn {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const float unit = big * (KV4_EVEN / KV4_WEIGHT);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int sh = 4; sh < 32; sh <<= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, sh);
 #pragma unroll
-      for (int sh = 4; sh < 32; sh <<= 1) {
-        l[n] += __shfl_xor_sync(0xffffffffu, l[n], sh);
-#pragma unroll
-        for (int j = 0; j < G; ++j) mo[n][j] += __shfl_xor_sync(0xffffffffu, mo[n][j], sh);
-      }
-      const int pr = it.tile * PAIRS + n * 4 + t;
-      if (pr >= it.q.T * gqa) continue;
-      T* out = static_cast<T*>(p.out) + ((size_t)(it.q.r0 + pr / gqa) * p.n_head + it.kv * gqa + pr % gqa) * HD;
-      float* dst = part + (size_t)(n * 4 + t) * PART;
-#pragma unroll
-      for (int sl = 0; sl < SLABS; ++sl)
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const float m = mo[n][sl * SG + b / 2];
-          const float4 x = sum_of(n, sl, b, 0), y = sum_of(n, sl, b, 1);
-          const float4 v = make_float4(fmaf(x.x + x.y, unit, m), fmaf(x.z + x.w, unit * 0.0625f, m),
-                                       fmaf(y.x + y.y, unit, m), fmaf(y.z + y.w, unit * 0.0625f, m));
-          const int d = sl * SLAB + b * 32 + g * 4;
-          if (part) *reinterpret_cast<float4*>(dst + 4 + d) = v;
-          else kv4_store4(out + d, kv4_quotient(v, l[n]));
-        }
-      if (part && g == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx[n], l[n]);
+      for (int j = 0; j < G; ++j) mo[j] += __shfl_xor_sync(0xffffffffu, mo[j], sh);
     }
+    const int pr = it.tile * PAIRS + t;
+    if (pr >= it.q.T * gqa) return;
+    T* out = static_cast<T*>(p.out) + ((size_t)(it.q.r0 + pr / gqa) * p.n_head + it.kv * gqa + pr % gqa) * HD;
+    float* dst = part + (size_t)t * PART;
+#pragma unroll
+    for (int sl = 0; sl < SLABS; ++sl)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const float m = mo[sl * SG + b / 2];
+        const float4 x = sum_of(sl, b, 0), y = sum_of(sl, b, 1);
+        const float4 v = make_float4(fmaf(x.x + x.y, unit, m), fmaf(x.z + x.w, unit * 0.0625f, m),
+                                     fmaf(y.x + y.y, unit, m), fmaf(y.z + y.w, unit * 0.0625f, m));
+        const int d = sl * SLAB + b * 32 + g * 4;
+        if (part) *reinterpret_cast<float4*>(dst + 4 + d) = v;
+        else kv4_store4(out + d, kv4_quotient(v, l));
+      }
+    if (part && g == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx, l);
   }
 };
 
-template <int HD, typename T, int NT>
-__global__ void __launch_bounds__(Kv4Attn<HD, NT>::NW * 32, 1) kv4_attend_kernel(const Kv4AttnParams p) {
-  using A = Kv4Attn<HD, NT>;
+template <int HD, typename T>
+__global__ void __launch_bounds__(Kv4Attn<HD>::NW * 32, 1) kv4_attend_kernel(const Kv4AttnParams p) {
+  using A = Kv4Attn<HD>;
   constexpr int PAIRS = A::PAIRS, NW = A::NW, E = HD / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
