@@ -300,7 +300,7 @@ struct Kv4Attn {
   float4* sums;
   bool flushed;
   float sco[4][2];            // the page's scores
-  int lim, lim_min, lim_max;  // the last position pair t sees (negative: none; no pair: all), and over the tile
+  int lim, lim_min, lim_max;  // the last position pair t sees (negative: none), and over the tile
 
   // The last position that any row of a tile sees.
   static FOX_DEV int last_seen(const Kv4Seq& q, int tile, int gqa) {
@@ -310,9 +310,9 @@ struct Kv4Attn {
   template <typename T>
   FOX_DEV void begin(const Kv4AttnParams& p, const Kv4Unit& it, int gqa) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    lim = it.tile * PAIRS + t < it.q.T * gqa ? it.q.at + (it.tile * PAIRS + t) / gqa : INT_MAX;
     lim_min = max(0, it.q.at + it.tile * PAIRS / gqa);
     lim_max = last_seen(it.q, it.tile, gqa);
+    lim = min(it.q.at + (it.tile * PAIRS + t) / gqa, lim_max);  // (no pair: as the tile)
     const float unit = p.scale * 1.44269504088896341f;
     const int pr = it.tile * PAIRS + (g >> 1);
     const bool live = pr < it.q.T * gqa;
@@ -370,7 +370,7 @@ struct Kv4Attn {
     l = 0.0f;
 #pragma unroll
     for (int j = 0; j < G; ++j) mo[j] = 0.0f;
-    big = 0x1p-24f;  // a power of two above every d met
+    big = 0x1p-24f;  // a power of two above every d that pair t met
     flushed = false;
   }
 
@@ -443,13 +443,28 @@ struct Kv4Attn {
     }
   }
 
+  // The largest finite d of a page's parameters: an infinite one makes its own
+  // group's sums what they are, and must not scale the others by it.
+  static FOX_DEV float largest_finite(const __half2 (&dv)[4][2][G]) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * G; ++i) {
+      const float d = __low2float(dv[i / (2 * G)][i / G % 2][i % G]);
+      if (!isinf(d)) most = fmaxf(most, d);
+    }
+#pragma unroll
+    for (int sh = 4; sh < 32; sh <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, sh));
+    return most;
+  }
+
   // Softmax weights of the page's scores and the sums over its V block. EDGE:
-  // some of its positions are hidden from some pair.
+  // some of its positions are hidden from some pair; those count as zeros for it,
+  // whatever the memory holds, in the scale of its weights too.
   template <bool EDGE>
   FOX_DEV void values(const uint8_t* vb, int pos0) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const __half2* dm = reinterpret_cast<const __half2*>(vb + kv4_codes_bytes(HD));
-    // this lane's parameters, the page's largest d, the maximum over its positions
+    // this lane's parameters, the largest d that pair t sees, and its largest score
     __half2 dv[4][2][G], most = __half2half2(__ushort_as_half(0));
     float top;
 #pragma unroll
@@ -457,14 +472,14 @@ struct Kv4Attn {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = s * 16 + h * 8 + g;
-        const bool nobody = EDGE && pos0 + at > lim_max;
+        const bool hidden = EDGE && pos0 + at > lim;
 #pragma unroll
         for (int j = 0; j < G; ++j) {
           dv[s][h][j] = dm[at * G + j];
-          if (nobody) dv[s][h][j] = __half2half2(__ushort_as_half(0));  // whatever the memory held
+          if (hidden) dv[s][h][j] = __half2half2(__ushort_as_half(0));
           most = __hmax2(most, dv[s][h][j]);
         }
-        if (EDGE && pos0 + at > lim) sco[s][h] = -INFINITY;
+        if (hidden) sco[s][h] = -INFINITY;
         top = s + h ? fmaxf(top, sco[s][h]) : sco[s][h];
       }
 #pragma unroll
@@ -472,10 +487,11 @@ struct Kv4Attn {
       most = __hmax2(most, __shfl_xor_sync(0xffffffffu, most, sh));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
     }
-    const float dmax = __low2float(most);
+    float dmax = __low2float(most);
     // The reference point of a pair's weights moves only when a score passes
     // it by 2^KV4_SLACK: the weights' scale leaves room for that.
     if (__any_sync(0xffffffffu, dmax >= big || top > mx + KV4_SLACK)) {
+      if (__any_sync(0xffffffffu, isinf(dmax))) dmax = largest_finite(dv);  // (NaN it passes over)
       const float to = dmax >= big ? __uint_as_float((__float_as_uint(dmax) & 0x7f800000u) + 0x00800000u) : big;
       const float shrink = big / to;
       big = to;
@@ -520,9 +536,8 @@ struct Kv4Attn {
         for (int j = 0; j < G; ++j) {
           const float2 d = __half22float2(dv[s][h][j]);
           const float m = fmaf(swap ? 15.0f - from_top : from_top, d.x, d.y);
-          const bool hidden = EDGE && sco[s][h] == -INFINITY;  // whatever it is
-          mo[j] = fmaf(w, hidden ? 0.0f : m, mo[j]);
-          pb[j][h] = transpose8x8(kv4_hi_lo(hidden ? 0.0f : wn * d.x));
+          mo[j] = fmaf(w, m, mo[j]);
+          pb[j][h] = transpose8x8(kv4_hi_lo(wn * d.x));
         }
       }
 #pragma unroll
