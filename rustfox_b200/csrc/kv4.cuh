@@ -48,21 +48,20 @@ struct Kv4Rows {
   int* err;
 };
 
-// The length of sequence s as given, and what of it its block table holds (less
-// is reported once per call of this).
-FOX_DEV int kv4_len(const Kv4Rows& c, int s) { return max(__ldg(c.kv_len + s), 0); }
-FOX_DEV int kv4_held(const Kv4Rows& c, int len) {
-  const int most = c.table_stride * KV_PAGE;
-  if (len > most && c.err) atomicExch(c.err, KERR_PAGES);
-  return min(len, most);
+FOX_DEV void kv4_outside(const Kv4Rows& c) {
+  if (c.err) atomicExch(c.err, KERR_PAGES);
 }
+
+// The length of sequence s as given, and what a block table holds.
+FOX_DEV int kv4_len(const Kv4Rows& c, int s) { return max(__ldg(c.kv_len + s), 0); }
+FOX_DEV int kv4_room(const Kv4Rows& c) { return c.table_stride * KV_PAGE; }
 
 // The page of sequence s that holds position p (inside the table), or -1
 // (reported) when the table names none of the cache's pages.
 FOX_DEV int kv4_page(const Kv4Rows& c, int s, int p) {
   const int page = __ldg(c.table + (size_t)s * c.table_stride + p / KV_PAGE);
   if ((unsigned)page < (unsigned)c.n_pages) return page;
-  if (c.err) atomicExch(c.err, KERR_PAGES);
+  kv4_outside(c);
   return -1;
 }
 
@@ -72,7 +71,7 @@ FOX_DEV int kv4_page(const Kv4Rows& c, int s, int p) {
 struct Kv4Place { int page, at; };
 FOX_DEV Kv4Place kv4_place(const Kv4Rows& c, int row) {
   Kv4Place x = {-1, 0};
-  if (row == c.n_rows - 1 && __ldg(c.row_start + c.n_seq) > c.n_rows && c.err) atomicExch(c.err, KERR_PAGES);
+  if (row == c.n_rows - 1 && __ldg(c.row_start + c.n_seq) > c.n_rows) kv4_outside(c);
   if (row >= c.n_rows || row < __ldg(c.row_start)) return x;
   int lo = 0, hi = c.n_seq;  // sequences that end at or before the row
   while (lo < hi) {
@@ -81,8 +80,9 @@ FOX_DEV Kv4Place kv4_place(const Kv4Rows& c, int row) {
   }
   if (lo >= c.n_seq) return x;
   const int pos = kv4_len(c, lo) - (__ldg(c.row_start + lo + 1) - row);
-  if (pos < 0 || kv4_held(c, pos + 1) <= pos) return x;
-  x.page = kv4_page(c, lo, pos);
+  if (pos < 0) return x;
+  if (pos < kv4_room(c)) x.page = kv4_page(c, lo, pos);
+  else kv4_outside(c);
   x.at = pos % KV_PAGE;
   return x;
 }

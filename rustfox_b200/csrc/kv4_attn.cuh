@@ -82,10 +82,9 @@ FOX_DEV Kv4Seq kv4_seq(const Kv4AttnParams& p, int s) {
   Kv4Seq q;
   q.r0 = min(max(__ldg(p.c.row_start + s), 0), p.c.n_rows);
   const int end = max(__ldg(p.c.row_start + s + 1), q.r0), len = kv4_len(p.c, s);
-  if (end > p.c.n_rows && p.c.err) atomicExch(p.c.err, KERR_PAGES);
   q.T = min(end, p.c.n_rows) - q.r0;
   q.at = len - (end - q.r0);
-  q.L = kv4_held(p.c, len);
+  q.L = min(len, kv4_room(p.c));
   q.tiles = (q.T * (p.n_head / p.c.n_kv) + PAIRS - 1) / PAIRS;
   q.units = KV4_HEAD + (q.L + KV_PAGE - 1) / KV_PAGE;
   return q;
@@ -111,8 +110,9 @@ struct Kv4Line {
   bool whole;  // no run is split between CTAs
   static __host__ __device__ int bytes(int n_seq) { return (2 * n_seq + 3) * 4; }
 
-  // By the CTA's first warp; every thread calls. A row_start that falls could
-  // count rows twice and the units past 2^31: it leaves the line empty.
+  // By the CTA's first warp; every thread calls. Lengths beyond the block table
+  // and rows beyond the row arrays are reported here. A row_start that falls
+  // could count rows twice and the units past 2^31: it leaves the line empty.
   template <int PAIRS>
   FOX_DEV void build(const Kv4AttnParams& p, void* mem) {
     n_seq = p.c.n_seq;
@@ -121,13 +121,15 @@ struct Kv4Line {
     const int lane = threadIdx.x & 31;
     if (threadIdx.x < 32) {
       int r0 = 0, u0 = 0, longest = 0;
-      bool falls = false;
+      bool outside = false, falls = false;
       for (int s0 = 0; s0 < n_seq; s0 += 32) {
         const int s = s0 + lane;
         int r = 0, n = 0;
         if (s < n_seq) {
           const Kv4Seq q = kv4_seq<PAIRS>(p, s);
-          falls = falls || __ldg(p.c.row_start + s + 1) < __ldg(p.c.row_start + s);
+          const int end = __ldg(p.c.row_start + s + 1);
+          falls = falls || end < __ldg(p.c.row_start + s);
+          outside = outside || falls || end > p.c.n_rows || kv4_len(p.c, s) > q.L;
           r = q.tiles * p.c.n_kv;
           n = r * q.units;
           if (r) longest = max(longest, q.units);
@@ -142,11 +144,11 @@ struct Kv4Line {
         r0 += __shfl_sync(0xffffffffu, rs, 31);
         u0 += __shfl_sync(0xffffffffu, ns, 31);
         if (__any_sync(0xffffffffu, falls)) {
-          if (lane == 0 && p.c.err) atomicExch(p.c.err, KERR_PAGES);
           r0 = u0 = 0;
           break;
         }
       }
+      if (outside) kv4_outside(p.c);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
       if (lane == 0) { run0[n_seq] = r0; unit0[n_seq] = u0; run0[n_seq + 1] = longest; }

@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
       if (leader) {
         bars.absent[loaded & 7] = !there;
         mbar_arrive_expect_tx(bar, there ? A::PAGE_BYTES : 0);
-        if (!there && p.c.err) atomicExch(p.c.err, KERR_PAGES);
+        if (!there) kv4_outside(p.c);
       }
       if (leader && there)
         bulk_g2s(smem + A::RAW_AT + (loaded % A::RAW) * A::PAGE_BYTES, kv4_block(p.c, next, lr.x.kv, 0, A::BB), A::PAGE_BYTES, bar);
