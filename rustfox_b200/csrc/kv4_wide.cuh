@@ -315,6 +315,10 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         const int e = min(max(7 - ((int)(__float_as_uint(top) >> 23) - 127), -100), 100);
         const float sc = __uint_as_float((uint32_t)(e + 127) << 23);
         f = p.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23);
+        // The score of a hidden position is -inf times f and a page's unit (2^-16
+        // at least), so their product must not fall to zero. No score that this
+        // changes exceeds 2^-60: the operands' products stay below 2^40.
+        f = fmaxf(f, 0x1p-100f);
 #pragma unroll
         for (int c = 0; c < OWN / 16; ++c) {
           constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
