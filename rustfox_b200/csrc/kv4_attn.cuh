@@ -40,6 +40,7 @@
 // the tiles of kv4_wide.cuh are faster.
 #pragma once
 
+#include <cfloat>
 #include <climits>
 
 #include "kv4.cuh"
@@ -224,6 +225,9 @@ FOX_DEV void kv4_operands(uint32_t x, uint32_t flip_e, uint32_t flip_o, uint32_t
 }
 constexpr float KV4_EVEN = 4194304.0f;  // 2^22
 constexpr int KV4_FLUSH = 4;  // pages whose sums stay in the matrix instructions' registers
+// Sums of a query's dimensions are held at this, so that no finite ones pass
+// fp32's range; what takes the scores of large queries back is held to it too.
+constexpr float KV4_QSUM = 1.0f / 64.0f;
 // A weight may exceed 1 by 2^SLACK before the sums are rescaled; times d it is
 // scaled to at most 2^15.
 constexpr float KV4_SLACK = 7.0f, KV4_WEIGHT = 256.0f;
@@ -331,19 +335,19 @@ struct Kv4Attn {
         x[j][4 * i] = v.x; x[j][4 * i + 1] = v.y; x[j][4 * i + 2] = v.z; x[j][4 * i + 3] = v.w;
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) { sum[j] += x[j][i]; top = fmaxf(top, fabsf(x[j][i])); }
+      for (int i = 0; i < 16; ++i) { sum[j] = fmaf(x[j][i], KV4_QSUM, sum[j]); top = fmaxf(top, fabsf(x[j][i])); }
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // the power of two that takes the largest |q| to [2^13, 2^14)
-    const int e = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -100), 100);
+    const int e = min(13 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
     const float sc = __uint_as_float((uint32_t)(e + 127) << 23);
-    const float back = unit * KV4_EVEN * __uint_as_float((uint32_t)(127 - e) << 23);
+    const float back = fminf(unit * KV4_EVEN * __uint_as_float((uint32_t)(127 - e) << 23), FLT_MAX);
     f = __shfl_sync(0xffffffffu, back, t * 8);
 #pragma unroll
-    for (int j = 0; j < G; ++j) qs[j] = __shfl_sync(0xffffffffu, sum[j], t * 8) * unit;
+    for (int j = 0; j < G; ++j) qs[j] = __shfl_sync(0xffffffffu, sum[j], t * 8) * (unit / KV4_QSUM);
     auto part = [&](float v, float by) {
       v *= sc * by;
       const float hi = __uint_as_float(__float_as_uint(v) & 0xffffe000u);

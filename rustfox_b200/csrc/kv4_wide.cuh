@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
           x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
         }
 #pragma unroll
-        for (int i = 0; i < OWN; ++i) { sum += x[i]; top = fmaxf(top, fabsf(x[i])); }
+        for (int i = 0; i < OWN; ++i) { sum = fmaf(x[i], KV4_QSUM, sum); top = fmaxf(top, fabsf(x[i])); }
         ex[share * PAIRS] = make_float4(sum, top, 0.0f, 0.0f);
         kv4_soft_sync();
 #pragma unroll
@@ -312,9 +312,9 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
           top = fmaxf(top, e.y);
         }
         // scaled by a power of two to below 2^8: a group's sum stays in range
-        const int e = min(max(7 - ((int)(__float_as_uint(top) >> 23) - 127), -100), 100);
+        const int e = min(7 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
         const float sc = __uint_as_float((uint32_t)(e + 127) << 23);
-        f = p.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23);
+        f = fminf(p.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - e) << 23), FLT_MAX);
         // The score of a hidden position is -inf times f and a page's unit (2^-16
         // at least), so their product must not fall to zero. No score that this
         // changes exceeds 2^-60: the operands' products stay below 2^40.
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
           __half h[2], l[2];
           h[1] = l[1] = __ushort_as_half(0);
 #pragma unroll
-          for (int g = 0; g < G; ++g) kv4_split(qs[g] * sc, &h[g], &l[g]);
+          for (int g = 0; g < G; ++g) kv4_split(qs[g] * (sc / KV4_QSUM), &h[g], &l[g]);
           const uint32_t m[8] = {half2_bits(__halves2half2(h[0], l[0])), half2_bits(__halves2half2(h[0], h[1])),
                                  half2_bits(__halves2half2(l[1], h[1])), 0, 0, 0, 0, 0};
           tmem_st8(tmem + lanes + A::QM_COL, m);

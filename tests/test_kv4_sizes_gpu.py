@@ -31,3 +31,32 @@ def test_scores_of_nothing_weigh_every_seen_position_alike(case, v, size, scale)
     want = R.attend(host(q.double()), c.data, c.table, [0, rows], [L], np.zeros((rows, heads, hd)), scale=scale)
     _close(got, want, "f32")
     rf.kernel_errors()
+
+
+@pytest.mark.parametrize("size,scale", [(1e33, 0.0), (1e35, 0.0), (1e36, 0.0), (1e36, 1e-36), (3e37, 1e-37), (3e37, 1e-30)])
+@pytest.mark.parametrize("case", CASES)
+def test_queries_near_the_end_of_fp32(case, size, scale):
+    """Finite queries give finite results: softmax's ordinary ones where the scale
+    makes up for their size, and otherwise the value whose score is the largest
+    (where no other comes within 2^-15 of the scores' size, the bound of
+    test_kv4_gpu.py 16 times over)."""
+    heads, kv, hd, rows, stride = case
+    L = 150
+    c = Cache([L], kv, hd, seed=4, stride=stride)
+    q = dev(size * c.rng.uniform(-1, 1, (rows, heads, hd))).float()
+    got = _attend(c, q, [rows], [L], scale=scale)
+    assert np.isfinite(got).all()
+    want = R.attend(host(q.double()), c.data, c.table, [0, rows], [L], np.zeros((rows, heads, hd)), scale=scale or None)
+    if size * scale and size * scale <= 10:
+        _close(got, want, "f32")
+        return
+    k = R.get(c.data, c.table, 0, np.arange(L))[0]
+    x = host(q.double()).reshape(rows, kv, heads // kv, hd)
+    z = np.einsum("rkgd,lkd->rkgl", x, k).reshape(rows, heads, L)
+    z[np.broadcast_to((np.arange(L) > L - rows + np.arange(rows)[:, None])[:, None], z.shape)] = -np.inf
+    top = np.sort(z, -1)[..., -2:]
+    most = np.einsum("rkgd,lkd->rkgl", np.abs(x), np.abs(k)).reshape(rows, heads, L).max(-1)
+    clear = top[..., 1] - top[..., 0] > 2.0 ** -15 * most
+    assert clear.mean() > 0.9
+    _close(got[clear], want[clear], "f32")
+    rf.kernel_errors()
