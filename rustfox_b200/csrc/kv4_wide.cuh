@@ -86,7 +86,7 @@ struct Kv4WideBars {
   float k_unit[4], v_unit[4];           // what 1 stands for in the page's operands
   unsigned v_bad[4][4];                 // positions whose V is not finite: [group][half of the page]
   int absent[8];                        // the block table names no page
-  unsigned seen[2][2][4];               // K's and V's warps: sizes in their parameters (1 not small, 2 large), 4 gave up
+  unsigned seen[2][2][4];               // K's and V's warps: the largest size of their parameters (its bits), all ones: gave up
   int dead;                             // a wait gave up
 };
 
@@ -188,11 +188,18 @@ FOX_DEV void kv4_split(float x, __half* hi, __half* lo) {
   *lo = __float2half_rn(x - __half2float(*hi));
 }
 // What a page's operands are scaled by, of the size |2 m + 15 d| + 15 |d| of its
-// largest group. Unscaled they are multiples of 2^-24, so that nothing is lost;
-// but large ones must stay below 2^16, and pages of small ones leave fp16's
-// subnormal numbers, for which the products' sums keep fewer bits.
-constexpr float KV4_LARGE = 32768.0f, KV4_SMALL = 1.0f / 16.0f;
-FOX_DEV float kv4_scale_of(int level) { return level == 0 ? 1.0f / 128.0f : level == 1 ? 1.0f : 65536.0f; }
+// largest group. Unscaled (level 2) they are multiples of 2^-24, and d c' loses
+// nothing; pages of small ones leave fp16's subnormal numbers, for which the
+// products' sums keep fewer bits (level 3). Large ones must stay below 2^16: with
+// values beyond 16384 (level 1) steps are rounded to multiples of 2^-22, so those
+// below 2^-12 lose bits; steps beyond 8736, which no write gives, are level 0.
+constexpr int KV4_LEVELS = 4;
+FOX_DEV int kv4_level(float size) {
+  return size < 1.0f / 16.0f ? 3 : size <= 32768.0f ? 2 : size <= 4.0f * 65504.0f ? 1 : 0;
+}
+FOX_DEV float kv4_scale_of(int level) {
+  return level == 3 ? 65536.0f : level == 2 ? 1.0f : level == 1 ? 1.0f / 4.0f : 1.0f / 128.0f;
+}
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const Kv4AttnParams p) {
@@ -503,7 +510,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
     bool ok = true;
     for (int u = a0; u < a1 && ok;) {
       const Part r = part_at(u);
-      int level = 2;  // V's only falls within a run: its sums have one scale
+      int level = KV4_LEVELS - 1;  // V's only falls within a run: its sums have one scale
       for (int page = r.first; page < r.last; ++page, ++j) {
         const int b = j & 1, left = r.lim_max - page * KV_PAGE;  // positions 0 .. left of the page are seen
         const uint8_t* raw = smem + A::RAW_AT + (j % A::RAW) * A::PAGE_BYTES + side * A::BB;
@@ -556,13 +563,13 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
         };
         // as the last page's, until all have been seen
         if (ok) store();
-        const unsigned seen = (__any_sync(0xffffffffu, top >= KV4_SMALL) ? 1u : 0u) | (__any_sync(0xffffffffu, top > KV4_LARGE) ? 2u : 0u);
-        if (lane == 0) bars.seen[side][b][warp & 3] = ok ? seen : 4u;
+        const unsigned seen = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // (never negative)
+        if (lane == 0) bars.seen[side][b][warp & 3] = ok ? seen : ~0u;
         sync();
         unsigned all = 0;
-        for (int k = 0; k < n / 32; ++k) all |= bars.seen[side][b][k];
-        if (all & 4) { ok = false; break; }
-        const int now = min(side ? level : 2, all & 2 ? 0 : all & 1 ? 1 : 2);
+        for (int k = 0; k < n / 32; ++k) all = max(all, bars.seen[side][b][k]);
+        if (all == ~0u) { ok = false; break; }
+        const int now = min(side ? level : KV4_LEVELS - 1, kv4_level(__uint_as_float(all)));
         if (now != level) {
           level = now;
           store();

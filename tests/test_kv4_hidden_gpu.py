@@ -52,7 +52,7 @@ def test_an_infinity_reaches_who_sees_it(case, what):
 
 
 @pytest.mark.parametrize("size", [1.0, 1e-2])
-@pytest.mark.parametrize("case", FEW)
+@pytest.mark.parametrize("case", FEW + MANY)
 def test_large_values_of_a_later_row_take_no_bits(case, size):
     """V of up to fp16's largest in the last position: steps of 8000 beside steps
     of 0.2, and of 0.002, which the rows before the last see."""
@@ -65,5 +65,24 @@ def test_large_values_of_a_later_row_take_no_bits(case, size):
     want = R.attend(host(q.double()), c.data, c.table, [0, rows], [L], np.zeros((rows, heads, hd)))
     assert R.get(c.data, c.table, 0, [L - 1])[1].max() > 5.9e4
     _close(got[:-1], want[:-1], "f32")
+    _close(got[-1:], want[-1:], "f32")
+    rf.kernel_errors()
+
+
+@pytest.mark.parametrize("case", FEW + MANY)
+def test_steps_that_no_write_gives(case):
+    """A cache filled by other means: finite steps of 60000 and offsets of fp16's
+    largest in one group of the last position, values of up to 965504."""
+    heads, kv, hd, rows, stride = case
+    c, q, L = _case(*case, seed=3)
+    n = 4 * (hd // R.GROUP)
+    o = R.PAGE * hd // 2 + (L - 1) % R.PAGE * n
+    for side in (0, 1):
+        blk = c.data[c.table[0, (L - 1) // R.PAGE], :, side]
+        blk[:, o:o + 4] = np.array([60000, 65504], np.float16).view(np.uint8)
+    got = _attend(c, q, [rows], [L])
+    want = R.attend(host(q.double()), c.data, c.table, [0, rows], [L], np.zeros((rows, heads, hd)))
+    _close(got[:-1], want[:-1], "f32")
+    # the last row's score there is beyond all others, above or below
     _close(got[-1:], want[-1:], "f32")
     rf.kernel_errors()
