@@ -106,8 +106,8 @@ foxcuda_status foxcuda_gemm_kq_i8(int ggml_type, const int8_t *q, const float *a
  * device error word per device (the outputs of that call are then not
  * valid); the calls on the 4-bit cache and foxcuda_qk_norm_rope below record
  * what their device arrays placed out of bounds there too.
- * foxcuda_kernel_errors synchronises the stream, reports the word
- * and clears it. The first tensor-core call on a device looks the word up;
+ * foxcuda_kernel_errors synchronises the stream, reports the word (a wait that
+ * gave up before positions that were skipped) and clears it. The first tensor-core call on a device looks the word up;
  * make it before any stream capture. */
 foxcuda_status foxcuda_kernel_errors(void *stream);
 /* The same on weights already packed by foxcuda_pack: no scratch. */

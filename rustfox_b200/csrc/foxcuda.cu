@@ -505,12 +505,7 @@ extern "C" foxcuda_status foxcuda_kernel_errors(void* stream) {
   CK(cudaMemcpy(&code, p, 4, cudaMemcpyDeviceToHost), "kernel_errors");
   if (!code) return FOXCUDA_OK;
   CK(cudaMemset(p, 0, 4), "kernel_errors");
-  if (code == KERR_PAGES)
-    return fail(FOXCUDA_ERR_ARG, "device: a call named a row, position or page outside its arrays (a position "
-                "beyond the tables, a cached length beyond the block table, a page outside the cache, a row_start "
-                "that falls or names more rows); what lay outside was skipped");
-  return fail(FOXCUDA_ERR_INTERNAL, "device: a bounded wait of a kernel-level tensor-core call gave up "
-              "(code %d); that call's output is not valid", code);
+  return kernel_err_status(code);
 }
 
 // ---------------------------------------------------------------------------

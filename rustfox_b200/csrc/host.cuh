@@ -80,8 +80,22 @@ inline cudaError_t opt_in_smem(K kern, size_t smem, size_t* marks) {
 // (foxcuda_kernel_errors reads and clears it); null when it cannot be found.
 int* kernel_err_ptr();
 
-// Its codes: a bounded wait that gave up, and a row, position or page that a
-// device-side array placed outside its bounds (the access was skipped).
+// Its codes: a bounded wait that gave up (or another code below 16 of a kernel
+// whose output is not valid), and the bit of a row, position or page that a
+// device-side array placed outside its bounds (the access was skipped). The bit
+// is added to what is there, and the graver code is what a call reports.
 enum KernelErr : int { KERR_WAIT = 1, KERR_PAGES = 16 };
+
+inline foxcuda_status kernel_err_status(int code) {
+  const char* outside =
+      "a call named a row, position or page outside its arrays (a position beyond the tables, a cached length beyond "
+      "the block table, a page outside the cache, a row_start that falls or names more rows); what lay outside was "
+      "skipped";
+  if (code & ~KERR_PAGES)
+    return fail(FOXCUDA_ERR_INTERNAL, "device: a bounded wait of a kernel-level tensor-core call gave up (code %d); "
+                "that call's output is not valid%s%s", code & ~KERR_PAGES, code & KERR_PAGES ? "; and " : "",
+                code & KERR_PAGES ? outside : "");
+  return code ? fail(FOXCUDA_ERR_ARG, "device: %s", outside) : FOXCUDA_OK;
+}
 
 }  // namespace fox

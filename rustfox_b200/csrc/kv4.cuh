@@ -49,7 +49,7 @@ struct Kv4Rows {
 };
 
 FOX_DEV void kv4_outside(const Kv4Rows& c) {
-  if (c.err) atomicExch(c.err, KERR_PAGES);
+  if (c.err) atomicOr(c.err, KERR_PAGES);
 }
 
 // The length of sequence s as given, and what a block table holds.
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const RopeParams p) {
 #pragma unroll
   for (int b = 0; b < BATCH; ++b) raw[b].load(x + (size_t)min(h0 + b * AT_ONCE, heads - 1) * HD);
   if (pos >= p.n_pos) {
-    if (lane == 0 && p.err) atomicExch(p.err, KERR_PAGES);
+    if (lane == 0 && p.err) atomicOr(p.err, KERR_PAGES);
     return;
   }
   float cs[C], sn[C];

@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(Kv4Attn<HD>::NW * 32, 1) kv4_attend_kernel(con
   auto arrived = [&](int side) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar + side, phase))) return;
     if (__any_sync(0xffffffffu, !mbar_wait(bar + side, phase))) {
-      if (lane == 0 && p.c.err) atomicExch(p.c.err, KERR_WAIT);
+      if (lane == 0 && p.c.err) atomicOr(p.c.err, KERR_WAIT);
       dead = true;
     }
   };

@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(Kv4Wide<HD>::THREADS, 1) kv4_wide_kernel(const
       }
       u = r.next;
     }
-    if (!ok && tid == 0 && p.c.err) atomicExch(p.c.err, KERR_WAIT);
+    if (!ok && tid == 0 && p.c.err) atomicOr(p.c.err, KERR_WAIT);
   } else if (warp < MMA_WARP) {
     // ---- a page's operands. Their loops stay rolled: four roles share a
     // scheduler's instruction cache, and copies of the bodies cost 6 %.
