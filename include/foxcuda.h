@@ -203,9 +203,10 @@ foxcuda_status foxcuda_attention(const float *q, const void *kcache, const void 
  *   rows as they were.
  * - head_dim 64, 128 or 256; at most 1024 sequences and 2^20 rows; the cache
  *   and the row arrays 16-byte aligned, row strides (in elements) a multiple
- *   of 16 bytes. No call allocates or synchronises, and each can be captured;
- *   the first call on a device looks up its error word, so make that before
- *   any capture. */
+ *   of 16 bytes. What a call writes must not overlap what it reads, or another
+ *   of its outputs (refused). No call allocates or synchronises, and each can
+ *   be captured; the first call on a device looks up its error word, so make
+ *   that before any capture. */
 typedef struct {
     void          *cache;
     const int32_t *table;      /* n_seq x table_stride */
@@ -251,8 +252,9 @@ foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4 *c, int ggml_type, const 
  * - A row with pos < 0 is padding: its outputs are left as they were. One with
  *   pos >= n_pos is skipped and reported by foxcuda_kernel_errors.
  * - q_out and k_out may be the rows of x that they come from (same strides),
- *   and must not overlap x or one another otherwise. Without norms the values
- *   are the decode step's rotation, bit for bit. */
+ *   and must not overlap what is read or one another otherwise (refused; rows
+ *   of the same stride may stand between one another's).
+ * - Without norms the values are the decode step's rotation, bit for bit. */
 foxcuda_status foxcuda_qk_norm_rope(int ggml_type, const void *x, size_t x_stride, uint32_t n_rows,
                                     uint32_t n_head, uint32_t n_head_kv, uint32_t head_dim,
                                     const float *q_norm, const float *k_norm, float eps,

@@ -6,7 +6,9 @@
 #include <cuda_runtime.h>
 
 #include <cstdarg>
+#include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/foxcuda.h"
@@ -76,6 +78,27 @@ inline cudaError_t opt_in_smem(K kern, size_t smem, size_t* marks) {
   return cudaSuccess;
 }
 
+// n rows of `row` bytes, `stride` bytes apart (memory without rows: one). None
+// where the pointer is null.
+struct Rows {
+  const void* p;
+  size_t row, n = 1, stride = 0;
+};
+// Rows of one stride may stand between one another's; of different strides their
+// whole ranges count.
+inline bool overlap(const Rows& a, const Rows& b) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  if (!x || !y || !a.n || !b.n || !a.row || !b.row) return false;
+  if (x >= y + (b.n - 1) * b.stride + b.row || y >= x + (a.n - 1) * a.stride + a.row) return false;
+  if (a.n < 2 || b.n < 2 || a.stride != b.stride) return true;
+  const size_t d = x < y ? (y - x) % a.stride : (a.stride - (x - y) % a.stride) % a.stride;  // from a row of a to the next of b
+  return d < a.row || d + b.row > a.stride;
+}
+inline bool overlap(const Rows& a, std::initializer_list<Rows> others) {
+  for (const Rows& b : others)
+    if (overlap(a, b)) return true;
+  return false;
+}
 // The device error word of kernel-level calls on the current device
 // (foxcuda_kernel_errors reads and clears it); null when it cannot be found.
 int* kernel_err_ptr();

@@ -30,9 +30,13 @@ static_assert(FOXCUDA_KV_PAGE == KV_PAGE, "the header's page size is the kernels
 static bool kv4_hd_ok(uint32_t hd) { return hd == 64 || hd == 128 || hd == 256; }
 static bool kv4_type_ok(int t) { return t == T_F32 || t == T_F16; }
 static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
-static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
-  return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+// The arrays that every call on a cache reads, and the cache.
+static Rows cache_of(const foxcuda_kv4* c) {
+  return {c->cache, (size_t)c->n_pages * c->n_head_kv * 2 * kv4_block_bytes((int)c->head_dim)};
 }
+static Rows table_of(const foxcuda_kv4* c) { return {c->table, (size_t)c->n_seq * c->table_stride * 4}; }
+static Rows starts_of(const foxcuda_kv4* c) { return {c->row_start, ((size_t)c->n_seq + 1) * 4}; }
+static Rows lens_of(const foxcuda_kv4* c) { return {c->kv_len, (size_t)c->n_seq * 4}; }
 static bool stride_ok(size_t stride, size_t row, int type) {
   return stride >= row && stride * (type == T_F32 ? 4 : 2) % 16 == 0 && stride <= ((size_t)1 << 32);
 }
@@ -101,6 +105,10 @@ extern "C" foxcuda_status foxcuda_kv4_write(const foxcuda_kv4* c, int type, cons
   if (!k || !v) return fail(FOXCUDA_ERR_ARG, "kv4_write: null pointer");
   if (!aligned16(k) || !aligned16(v) || !stride_ok(k_stride, row, type) || !stride_ok(v_stride, row, type))
     return fail(FOXCUDA_ERR_ARG, "kv4_write: rows must be 16-byte aligned and at least a row apart");
+  const size_t size = type == T_F32 ? 4 : 2;
+  if (overlap(cache_of(c), {{k, row * size, c->n_rows, k_stride * size}, {v, row * size, c->n_rows, v_stride * size},
+                            table_of(c), starts_of(c), lens_of(c)}))
+    return fail(FOXCUDA_ERR_ARG, "kv4_write: the cache overlaps what is read");
   p.k = const_cast<void*>(k); p.v = const_cast<void*>(v); p.k_stride = k_stride; p.v_stride = v_stride;
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
        return by_rows<hd.value>(p.c, [&](auto rows, unsigned grid) {
@@ -118,7 +126,9 @@ extern "C" foxcuda_status foxcuda_kv4_read(const foxcuda_kv4* c, int type, void*
   if (!k || !v) return fail(FOXCUDA_ERR_ARG, "kv4_read: null pointer");
   if (!aligned16(k) || !aligned16(v)) return fail(FOXCUDA_ERR_ARG, "kv4_read: rows must be 16-byte aligned");
   const size_t bytes = (size_t)c->n_rows * c->n_head_kv * c->head_dim * (type == T_F32 ? 4 : 2);
-  if (overlap(k, bytes, v, bytes)) return fail(FOXCUDA_ERR_ARG, "kv4_read: the outputs overlap");
+  if (overlap(Rows{k, bytes}, {{v, bytes}, cache_of(c), table_of(c), starts_of(c), lens_of(c)}) ||
+      overlap(Rows{v, bytes}, {cache_of(c), table_of(c), starts_of(c), lens_of(c)}))
+    return fail(FOXCUDA_ERR_ARG, "kv4_read: the outputs overlap one another or what is read");
   p.k = k; p.v = v;
   CK(by_type_hd(type, c->head_dim, [&](auto tag, auto hd) {
        return by_rows<hd.value>(p.c, [&](auto rows, unsigned grid) {
@@ -165,6 +175,16 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
       (q_norm && !aligned16(q_norm)) || (k_norm && !aligned16(k_norm)) || !stride_ok(x_stride, nq + nk, type) ||
       !stride_ok(q_stride, nq, type) || !stride_ok(k_stride, nk, type))
     return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: rows and tables must be 16-byte aligned, rows at least a row apart");
+  const size_t size = type == T_F32 ? 4 : 2;
+  const Rows xq = {x, nq * size, n_rows, x_stride * size}, xk = {(const char*)x + nq * size, nk * size, n_rows, x_stride * size};
+  const Rows qo = {q_out, nq * size, n_rows, q_stride * size}, ko = {k_out, nk * size, n_rows, k_stride * size};
+  const Rows angles[3] = {{cos, (size_t)n_pos * (head_dim / 2) * 4}, {sin, (size_t)n_pos * (head_dim / 2) * 4}, {pos, (size_t)n_rows * 4}};
+  const Rows norms[2] = {{q_norm, (size_t)head_dim * 4}, {k_norm, (size_t)head_dim * 4}};
+  const auto in_place = [&](const Rows& out, const Rows& in) { return out.p == in.p && (out.stride == in.stride || n_rows == 1); };
+  if ((!in_place(qo, xq) && overlap(qo, xq)) || (!in_place(ko, xk) && overlap(ko, xk)) ||
+      overlap(qo, {ko, xk, angles[0], angles[1], angles[2], norms[0], norms[1]}) ||
+      overlap(ko, {xq, angles[0], angles[1], angles[2], norms[0], norms[1]}))
+    return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: the outputs overlap one another or what is read (each may be its own rows of x)");
   RopeParams p{};
   p.x = x; p.pos = pos; p.q_norm = q_norm; p.k_norm = k_norm; p.cos = cos; p.sin = sin; p.q = q_out; p.k = k_out;
   p.x_stride = x_stride; p.q_stride = q_stride; p.k_stride = k_stride;
@@ -256,8 +276,11 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
       !stride_ok(q_stride, (size_t)n_head * c->head_dim, type))
     return fail(FOXCUDA_ERR_ARG, "kv4_attention: rows and workspace must be 16-byte aligned, rows at least a row apart");
   const size_t size = type == T_F32 ? 4 : 2, row = (size_t)n_head * c->head_dim;
-  if (overlap(q, ((c->n_rows - 1) * q_stride + row) * size, out, c->n_rows * row * size))
-    return fail(FOXCUDA_ERR_ARG, "kv4_attention: q and out overlap");
+  const Rows queries = {q, row * size, c->n_rows, q_stride * size};
+  if (overlap(Rows{out, c->n_rows * row * size},
+              {queries, {workspace, need}, cache_of(c), table_of(c), starts_of(c), lens_of(c)}) ||
+      overlap(Rows{workspace, need}, {queries, cache_of(c), table_of(c), starts_of(c), lens_of(c)}))
+    return fail(FOXCUDA_ERR_ARG, "kv4_attention: out or the workspace overlap what is read, or one another");
   // tiles of at least 4 (row, head) pairs, each with every page of its sequence
   const double units = ((double)c->n_rows * gqa / 4 + c->n_seq) * c->n_head_kv * ((double)c->table_stride + KV4_HEAD);
   if (units >= 2147483648.0)
