@@ -414,7 +414,8 @@ def _kv4(what: str, cache, table, row_start, kv_len, n_rows: int):
 
 def _rows(what: str, name: str, t, n_rows: int, heads: int, hd: int, dtype) -> int:
     """t as n_rows rows of heads * hd values ([rows, heads * hd] or [rows,
-    heads, hd], each row contiguous): its row stride in elements."""
+    heads, hd], each row contiguous): its row stride in elements (a single row
+    has none, whatever tensor it is a slice of)."""
     shape, stride = t.shape, t.stride()
     if len(shape) == 2:
         ok = shape[1] == heads * hd and stride[1] == 1
@@ -423,7 +424,7 @@ def _rows(what: str, name: str, t, n_rows: int, heads: int, hd: int, dtype) -> i
     if not ok or shape[0] != n_rows or t.dtype is not dtype:
         _bad(what, f"{name} holds {n_rows} {dtype} rows of {heads} x {hd} values, each row contiguous; "
                    f"got {t.dtype} {tuple(shape)}")
-    return stride[0] if n_rows > 1 else max(stride[0], heads * hd)
+    return stride[0] if n_rows > 1 else heads * hd
 
 
 def kv4_write(cache, table, row_start, kv_len, k, v):
@@ -537,7 +538,7 @@ def qk_norm_rope(x, n_head: int, n_head_kv: int, head_dim: int, pos, cos, sin, q
         if w is not None and (w.dtype is not f32 or w.shape != (head_dim,) or not w.is_contiguous()):
             _bad(what, f"the norm weights are contiguous float32 tensors of {head_dim} values")
     _call_on(what, lib().foxcuda_qk_norm_rope,
-             (_row_type(what, dtype), x.data_ptr(), stride[0] if n > 1 else max(stride[0], nq + nk), n, n_head,
+             (_row_type(what, dtype), x.data_ptr(), stride[0] if n > 1 else nq + nk, n, n_head,
               n_head_kv, head_dim, None if q_norm is None else q_norm.data_ptr(),
               None if k_norm is None else k_norm.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), n_pos, halves,
               pos.data_ptr(), q_out.data_ptr(), qs, k_out.data_ptr(), ks),
