@@ -228,7 +228,7 @@ foxcuda_status foxcuda_kv4_read(const foxcuda_kv4 *c, int ggml_type, void *k, vo
 /* Each row's n_head query heads over positions 0..its own of its sequence
  * (upstream attention_heads, src/forward.c:222-257, for many rows): q and out
  * are rows of n_head * head_dim FOXCUDA_F32 or FOXCUDA_F16 values, q's
- * q_stride elements apart; they must not overlap. n_head / n_head_kv is 1, 2, 4 or 8; scale
+ * q_stride elements apart; they must not overlap. n_head / n_head_kv is 1 to 8; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). The sums and softmax
  * statistics are fp32. The same call gives the same bits; a row's sums are
  * split where an even division of the call's pages falls, so its last bits

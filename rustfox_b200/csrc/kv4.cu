@@ -266,7 +266,7 @@ extern "C" foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4* c, int type, 
   foxcuda_status st = check_kv4(c, type, "kv4_attention", &p.c, &none);
   if (st) return st;
   const uint32_t gqa = n_head / c->n_head_kv;
-  if (!n_head || n_head > 1024 || n_head % c->n_head_kv || (gqa != 1 && gqa != 2 && gqa != 4 && gqa != 8))
+  if (!n_head || n_head > 1024 || n_head % c->n_head_kv || gqa > 8)
     return fail(FOXCUDA_ERR_UNSUPPORTED, "kv4_attention: %u heads over %u KV heads are not covered", n_head, c->n_head_kv);
   if (!(scale >= 0.0f) || scale > 3.0e38f) return fail(FOXCUDA_ERR_ARG, "kv4_attention: scale %g", (double)scale);
   if (none) return FOXCUDA_OK;
