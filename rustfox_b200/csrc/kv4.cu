@@ -30,6 +30,7 @@ static_assert(FOXCUDA_KV_PAGE == KV_PAGE, "the header's page size is the kernels
 static bool kv4_hd_ok(uint32_t hd) { return hd == 64 || hd == 128 || hd == 256; }
 static bool kv4_type_ok(int t) { return t == T_F32 || t == T_F16; }
 static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+static bool aligned4(const void* p) { return (uintptr_t)p % 4 == 0; }
 // The arrays that every call on a cache reads, and the cache.
 static Rows cache_of(const foxcuda_kv4* c) {
   return {c->cache, (size_t)c->n_pages * c->n_head_kv * 2 * kv4_block_bytes((int)c->head_dim)};
@@ -61,6 +62,8 @@ static foxcuda_status check_kv4(const foxcuda_kv4* c, int type, const char* what
   if (*none) return FOXCUDA_OK;
   if (!c->cache || !c->table || !c->row_start || !c->kv_len) return fail(FOXCUDA_ERR_ARG, "%s: null pointer", what);
   if (!aligned16(c->cache)) return fail(FOXCUDA_ERR_ARG, "%s: the cache must be 16-byte aligned", what);
+  if (!aligned4(c->table) || !aligned4(c->row_start) || !aligned4(c->kv_len))
+    return fail(FOXCUDA_ERR_ARG, "%s: table, row_start and kv_len must be 4-byte aligned", what);
   r->cache = static_cast<uint8_t*>(c->cache);
   r->table = c->table; r->row_start = c->row_start; r->kv_len = c->kv_len;
   r->n_pages = (int)c->n_pages; r->n_kv = (int)c->n_head_kv; r->n_seq = (int)c->n_seq;
@@ -170,6 +173,7 @@ extern "C" foxcuda_status foxcuda_qk_norm_rope(int type, const void* x, size_t x
     return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: %u rows / %u positions", n_rows, n_pos);
   if (n_rows == 0) return FOXCUDA_OK;
   if (!x || !cos || !sin || !pos || !q_out || !k_out) return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: null pointer");
+  if (!aligned4(pos)) return fail(FOXCUDA_ERR_ARG, "qk_norm_rope: pos must be 4-byte aligned");
   const size_t nq = (size_t)n_head * head_dim, nk = (size_t)n_head_kv * head_dim;
   if (!aligned16(x) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(cos) || !aligned16(sin) ||
       (q_norm && !aligned16(q_norm)) || (k_norm && !aligned16(k_norm)) || !stride_ok(x_stride, nq + nk, type) ||
