@@ -228,14 +228,24 @@ foxcuda_status foxcuda_kv4_read(const foxcuda_kv4 *c, int ggml_type, void *k, vo
 /* Each row's n_head query heads over positions 0..its own of its sequence
  * (upstream attention_heads, src/forward.c:222-257, for many rows): q and out
  * are rows of n_head * head_dim FOXCUDA_F32 or FOXCUDA_F16 values, q's
- * q_stride elements apart; they must not overlap. n_head / n_head_kv is 1 to 8; scale
- * multiplies the scores (0: 1 / sqrt(head_dim)). The sums and softmax
- * statistics are fp32. The same call gives the same bits; a row's sums are
- * split where an even division of the call's pages falls, so its last bits
- * can differ beside other sequences. workspace holds
- * foxcuda_kv4_attention_workspace() bytes of the current device (16-byte
- * aligned; need not be initialised; NULL where that is 0, for block tables of
- * up to 16 pages); calls that may run at the same time must not share it. */
+ * q_stride elements apart. n_head / n_head_kv is 1 to 8; scale multiplies the
+ * scores (0: 1 / sqrt(head_dim)).
+ * - The sums and softmax statistics are fp32; queries, weights and what is
+ *   cached enter the matrix products as pairs of fp16 numbers, 22 bits. A score
+ *   z is off by up to about 2^-19 |z|; fp32 results with ordinary scores are
+ *   within some 1e-6 of the exact ones' norm. For many rows, steps below 2^-12
+ *   beside values beyond 16384 (K: in a page, V: in the pages up to them) are
+ *   held to 2^-23.
+ * - The same call gives the same bits; a row's sums are split where an even
+ *   division of the call's pages falls, so its last bits can differ beside other
+ *   sequences.
+ * - One of two kernels serves a call, by its average of rows a sequence, padding
+ *   included: chunks of many rows and single tokens behind long contexts are
+ *   faster as two calls.
+ * - workspace holds foxcuda_kv4_attention_workspace() bytes of the current
+ *   device (16-byte aligned; need not be initialised; NULL where that is 0, for
+ *   block tables of up to 16 pages); calls that may run at the same time must
+ *   not share it. */
 size_t         foxcuda_kv4_attention_workspace(uint32_t head_dim, uint32_t table_stride);
 foxcuda_status foxcuda_kv4_attention(const foxcuda_kv4 *c, int ggml_type, const void *q, size_t q_stride,
                                      uint32_t n_head, float scale, void *workspace,

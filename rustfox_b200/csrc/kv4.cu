@@ -18,11 +18,19 @@ using namespace fox;
 // head) pairs a sequence and KV head on: their time hardly depends on the rows.
 // 4 sequences of 16384 positions, 8 KV heads of 128: 32 pairs 120 us either way,
 // 48 pairs 170 us narrow and 121 wide, 128 pairs 423 and 130; of 64: 32 pairs 77
-// and 83, 48 pairs 110 and 84.
+// and 83, 48 pairs 110 and 84. The rule sees what the host knows, a call's average
+// with its padding rows, so a call of unlike sequences can be better as two: 64
+// rows beside 15 single tokens, 16384 positions each, take 268 us in one call and
+// 85 + 67 in two; 16 tokens of 4096 positions take 33 us, in 1024 row places 137.
+// Heads of 256 dimensions stay with the narrow tiles (64 rows of 16 heads over 4
+// behind 8192 positions: 134 us): S of two pages, O with the offsets and both
+// halves of q would take 664 of tensor memory's 512 columns.
 constexpr int KV4_WIDE_FROM = 48;
 // Where no run is split, a tile has one SM for its pages, so there must also be
 // this many pairs an SM: one sequence of 1000 positions, 128 pairs for each of 8
-// KV heads, 18 us narrow and 42 wide; 16 of 512, 48 pairs, 41 and 27.
+// KV heads, 18 us narrow and 42 wide; 16 of 512, 48 pairs, 41 and 27. (A longer
+// table may hold short sequences all the same: 128 pairs behind 1000 positions
+// under one of 512 pages take 47 us.)
 constexpr int KV4_WIDE_FILL = 32;
 
 static_assert(FOXCUDA_KV_PAGE == KV_PAGE, "the header's page size is the kernels'");
@@ -86,9 +94,9 @@ static cudaError_t by_type_hd(int type, uint32_t hd, F f) {
 }
 
 // One row a warp where the rows are few, so that they spread over the device (16
-// written: 6.0 us, 8.7 with four rows a warp); four, for one search for their
-// places and more loads in flight, where they fill it anyway (32768 read: 39 us,
-// 72 with one; 4616 written: 22 and 23).
+// fp32 rows written: 2.7 us, 4.1 with four rows a warp; read 2.9 and 4.3); four,
+// for one search for their places and more loads in flight, where they fill it
+// anyway (32768 read to fp16: 39 us, 71 with one; 4616 written: 13.7 and 15.0).
 template <int HD, typename F>
 static cudaError_t by_rows(const Kv4Rows& c, F f) {
   const int passes = Kv4Pass<HD>::passes(c.n_kv);
@@ -149,7 +157,7 @@ static cudaError_t launch_rope_b(const RopeParams& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 // One load a warp where the rows are few, so that they spread over the device (1
-// row of 40 heads: 1.7 us, 2.3 with four); four, each row's tables loaded once
+// row of 40 heads: 1.6 us, 2.2 with four); four, each row's tables loaded once
 // for them, where they fill it anyway (4096 fp16 rows of 48 heads: 23 us, 38 with
 // one).
 template <typename T, int HD, bool HALVES>

@@ -277,9 +277,14 @@ FOX_DEV Kv4Place kv4_places(const Kv4Rows& c, int row0) {
 constexpr int KV4_AT_ONCE = 4;  // rows whose loads are in flight together
 
 // Quantises rows into their positions: a group's minimum and maximum over the 8
-// lanes that hold it, then every lane's codes. Bound by its instructions, some
-// 25 a value for the exact codes: 4616 fp32 rows of 8 heads of 128 take 22 us
-// (2.4 TB/s of values read and codes written). A step's 16 rows take 5.9 us: a
+// lanes that hold it, then every lane's codes. Bound by its instructions, 26 a
+// value for the exact codes (28 from fp16, where one warp's groups in twelve hold
+// a value on the border of two codes and take the careful form), and by the wait
+// for a warp's rows in front of them, which few warps overlap: 4616 fp32 rows of
+// 8 heads of 128 take 13.8 us (43 MB of values read and codes written, 3.1 TB/s)
+// with 56 % of the issue slots, 32768 65 us (4.7 TB/s), 32768 from fp16 75 us
+// (2.3 TB/s, 74 % of the slots). Padding rows are read before it is known that
+// they are: 2808 rows among 4616 take 12.1 us. A step's 16 rows take 2.7 us: a
 // launch, and the dependent loads of row, length and page.
 template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4MoveParams p) {
@@ -335,8 +340,10 @@ FOX_DEV void kv4_decode(uint32_t code, __half2 pair, float (&v)[8]) {
   }
 }
 
-// The rows' values, x = m + d c with one rounding. Bound by the writes that it
-// must make: 32768 positions of 8 heads of 128 to fp16 take 39 us, 4.4 TB/s.
+// The rows' values, x = m + d c with one rounding. Bound by its instructions, 15
+// a value with their addresses (76 % of the issue slots), before the memory: 32768
+// positions of 8 heads of 128 to fp16 take 39 us, 4.4 TB/s, to fp32 64 us, 4.8
+// TB/s.
 template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4MoveParams p) {
   griddep_wait();
@@ -432,9 +439,11 @@ FOX_DEV void rope_store(__half* p, const float (&v)[8]) { kv4_store8(p, v); }
 // apart. A warp takes BATCH such loads of one row's query or key heads, so that
 // the row's sines, cosines and the weights are loaded once for all of them and
 // the loads are in flight together. Without norms the result is that of the
-// decode step's rotation, bit for bit. Bound by memory where there is work:
-// 4096 fp16 rows of 32 + 16 heads of 128 take 23 us, 4.5 TB/s; 1 to 100 rows
-// take 1.6 us, a launch.
+// decode step's rotation, bit for bit. fp32 rows are bound by memory: 4096 of 32 +
+// 8 heads of 128 take 28 us, 6.1 TB/s. fp16 rows, with twice the arithmetic a
+// byte, are bound by their instructions (66 % of the issue slots, the rest waits
+// for loads and exchanges): 4096 of 32 + 16 heads take 23 us, 4.5 TB/s. 1 to 100
+// rows take 1.6 us, a launch.
 template <typename T, int HD>
 struct RopeLay {
   static constexpr int E = sizeof(T) == 2 || HD == 256 ? 8 : 4, LANES = HD / E, AT_ONCE = 32 / LANES;

@@ -31,12 +31,12 @@
 //   positions, now it is 1e-6.
 //
 // Bound by memory for long single tokens, with the issue of instructions close
-// behind: 16 sequences of 32768 positions, 32 heads over 8 of 128, take 122 us,
-// 4.9 TB/s of codes and parameters; 64 ragged fp16 ones over 16 KV heads 129 us,
+// behind: 16 sequences of 32768 positions, 32 heads over 8 of 128, take 120 us,
+// 5.0 TB/s of codes and parameters; 64 ragged fp16 ones over 16 KV heads 128 us,
 // 4.7 TB/s. Short ones are bound by their chain of dependent loads (row, length,
 // page, codes) and the launch: 576 positions 11 us, 65 positions 8 us. With many
 // rows the products and the weights of every row bound it: 32 (row, head) pairs
-// for each of 8 KV heads, 4 sequences of 8192 positions, 71 us; from 48 pairs on
+// for each of 8 KV heads, 4 sequences of 8192 positions, 69 us; from 48 pairs on
 // the tiles of kv4_wide.cuh are faster.
 #pragma once
 

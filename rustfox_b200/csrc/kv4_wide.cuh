@@ -6,8 +6,8 @@
 // d c' has 15 significant bits, so it is hi + lo in fp16 exactly (a product and
 // the fused remainder), and the offsets 2 m + 15 d, one for each position and
 // group, are hi + lo to 22 bits. So the unpacked page is a set of fp16
-// operands, scaled by a power of two to fp16's range, and the parameters never
-// meet the scores:
+// operands, scaled by a power of two to fp16's range (kv4_level says what that
+// costs beside values beyond 16384), and the parameters never meet the scores:
 //   S = Qh Kh + Ql Kh + Qh Kl + (sums of q per group) (offsets of K)
 //   O = Ph Vh + Pl Vh + Ph Vl,  with V's offsets as further columns
 // with q and the weights as hi + lo fp16 too. (An earlier form multiplied the
@@ -30,7 +30,7 @@
 //   0.6 % of the time less at every 8.
 // The work is divided as in kv4_attn.cuh, with a CTA for a warp.
 //
-// 64 rows behind 16384 positions, 32 heads over 8 of 128, take 84 us: 205
+// 64 rows behind 16384 positions, 32 heads over 8 of 128, take 83 us: 207
 // TFLOP/s of the formula's products, of which this form issues three for one and
 // the offsets. A page takes a tile about 4300 cycles, and K's three warps are
 // what it waits for (1200 cycles for the parameters and their exchange, 1800 for
